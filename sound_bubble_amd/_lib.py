@@ -256,6 +256,62 @@ SYMBOLS = {
     "sb_l1_grad": (_ci, [c_fp, c_fp, i64, _cf, c_fp, _ci, c_fp, _cf, c_fp, _ci, _vp]),
 }
 
+# ---- include/sound_bubble_seq.h: layer norm, gated linear recurrence, AdamW over many tensors ----
+class LayerNormArgs(C.Structure):
+    _fields_ = [("rows", i64), ("n", i64), ("ldx", i64), ("xtype", C.c_int), ("wtype", C.c_int), ("eps", C.c_float),
+                ("x", C.c_void_p), ("w", C.c_void_p), ("b", C.c_void_p), ("y", C.c_void_p), ("mean", c_fp), ("rstd", c_fp)]
+
+
+class LayerNormBwdArgs(C.Structure):
+    _fields_ = [("rows", i64), ("n", i64), ("ldx", i64), ("lddy", i64), ("xtype", C.c_int), ("wtype", C.c_int),
+                ("x", C.c_void_p), ("dy", C.c_void_p), ("w", C.c_void_p), ("mean", c_fp), ("rstd", c_fp),
+                ("dx", C.c_void_p), ("dw", C.c_void_p), ("db", C.c_void_p), ("scratch", c_fp)]
+
+
+class GatedScanArgs(C.Structure):
+    _fields_ = [("outer", i64), ("steps", i64), ("inner", i64),
+                ("xtype", C.c_int), ("gtype", C.c_int), ("form", C.c_int), ("reverse", C.c_int),
+                ("x", C.c_void_p), ("so_x", i64), ("st_x", i64), ("gate", C.c_void_p), ("so_g", i64), ("st_g", i64),
+                ("h0", c_fp), ("len", C.c_void_p), ("h", C.c_void_p), ("h_last", c_fp), ("states", c_fp), ("scratch", c_fp)]
+
+
+class GatedScanBwdArgs(C.Structure):
+    _fields_ = [("outer", i64), ("steps", i64), ("inner", i64),
+                ("xtype", C.c_int), ("gtype", C.c_int), ("form", C.c_int), ("reverse", C.c_int),
+                ("x", C.c_void_p), ("so_x", i64), ("st_x", i64), ("gate", C.c_void_p), ("so_g", i64), ("st_g", i64),
+                ("dh", C.c_void_p), ("so_d", i64), ("st_d", i64), ("dlast", c_fp), ("len", C.c_void_p), ("states", c_fp),
+                ("dx", C.c_void_p), ("dgate", C.c_void_p), ("dh0", c_fp), ("scratch", c_fp)]
+
+
+ADAMW_BLOCK, ADAMW_MAX, ADAMW_NORM_SLOTS = 256, 112, 512
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("n", i64), ("first_block", C.c_int32), ("first_chunk", C.c_int32)]
+
+
+class AdamwArgs(C.Structure):
+    _fields_ = [("t", AdamwTensor * ADAMW_MAX), ("count", C.c_int32), ("ptype", C.c_int32), ("gtype", C.c_int32), ("bits", C.c_int32),
+                ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("master", c_fp),
+                ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("lr_dev", c_fp), ("step_dev", C.c_void_p), ("step", C.c_int32), ("seed", C.c_uint32),
+                ("gscale", C.c_float), ("clip", C.c_float), ("norm_part", C.c_void_p), ("norm_slots", C.c_int32),
+                ("guard", C.c_void_p), ("skipped", C.c_void_p), ("last", C.c_int32)]
+
+
+SEQ_SYMBOLS = {
+    "sb_layer_norm_fwd": (_ci, [C.POINTER(LayerNormArgs), _vp]),
+    "sb_layer_norm_bwd_scratch": (i64, [i64, i64, _ci]),
+    "sb_layer_norm_bwd": (_ci, [C.POINTER(LayerNormBwdArgs), _vp]),
+    "sb_gated_scan_plan": (_ci, [i64, i64, i64, _ci, C.POINTER(i64), C.POINTER(i64), C.POINTER(i64)]),
+    "sb_gated_scan_fwd": (_ci, [C.POINTER(GatedScanArgs), _vp]),
+    "sb_gated_scan_bwd": (_ci, [C.POINTER(GatedScanBwdArgs), _vp]),
+    "sb_gated_scan_step": (_ci, [_vp, _vp, _vp, _vp, i64, i64, i64, i64, _ci, _ci, _ci, _vp]),
+    "sb_adamw_chunk": (_ci, []),
+    "sb_adamw_norm": (_ci, [C.POINTER(AdamwArgs), _vp, _ci, _ci, _vp]),
+    "sb_adamw_step": (_ci, [C.POINTER(AdamwArgs), _vp]),
+}
+
 _lib = None
 
 
@@ -273,7 +329,7 @@ def load():
             f"{LIB_PATH} is missing. Build it with `python -m sound_bubble_amd.build` "
             "(hipcc --offload-arch=gfx950). There is no CPU / eager fallback for the hot path.")
     lib = C.CDLL(LIB_PATH)
-    for name, (res, args) in SYMBOLS.items():
+    for name, (res, args) in {**SYMBOLS, **SEQ_SYMBOLS}.items():
         fn = getattr(lib, name)       # AttributeError if the .so does not export it
         fn.restype = res
         fn.argtypes = args

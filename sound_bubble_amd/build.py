@@ -9,8 +9,13 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libsoundbubble_hip.so")
 SOURCES = ["sb_lstm.hip", "sb_lstm_gen.hip", "sb_lstm_vec.hip", "sb_lstm_bf_fwd.hip", "sb_lstm_bf_bwd.hip", "sb_lstm_stream.hip", "sb_attention.hip",
            "sb_linear.hip", "sb_elementwise.hip", "sb_mrstft.hip"]
+# the sequence-block operators (layer norm, gated linear recurrence, AdamW): a folder and a header of their own, so that the digest
+# below stays the separator kernels'
+SEQ_SOURCES = ["seq/sb_layer_norm.hip", "seq/sb_gated_scan.hip", "seq/sb_adamw.hip"]
 HEADERS = [os.path.join(CSRC, "sb_common.h"), os.path.join(CSRC, "sb_lstm_bf_common.h"),
            os.path.join(HERE, "..", "include", "sound_bubble_hip.h")]
+SEQ_HEADERS = [os.path.join(CSRC, "sb_common.h"), os.path.join(CSRC, "seq", "sb_seq_common.h"),
+               os.path.join(HERE, "..", "include", "sound_bubble_seq.h")]
 
 
 def csrc_digest():
@@ -38,7 +43,12 @@ def _stale(target, deps):
 # -ffp-contract=off: every fused multiply-add in the recurrent kernels is written out (__builtin_fmaf), so all template
 # variants of a kernel (e.g. the time-segmented and the plain schedule) round identically -- bit-exact outputs.
 _BF_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form", "-ffp-contract=off"]
-PER_FILE_FLAGS = {"sb_lstm_bf_fwd.hip": _BF_FLAGS, "sb_lstm_bf_bwd.hip": _BF_FLAGS}
+# no packed fp32 instructions in the sequence-block kernels: they wait for memory, and those forms are not needed for it; AdamW
+# rounds every operation by itself (its 8-bit codes are defined by those roundings)
+_SEQ_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+PER_FILE_FLAGS = {"sb_lstm_bf_fwd.hip": _BF_FLAGS, "sb_lstm_bf_bwd.hip": _BF_FLAGS,
+                  "seq/sb_layer_norm.hip": _SEQ_FLAGS, "seq/sb_gated_scan.hip": _SEQ_FLAGS,
+                  "seq/sb_adamw.hip": _SEQ_FLAGS + ["-ffp-contract=off"]}
 # translation units built a second time with another macro set: (source, object stem, extra flags).  The opt-in two-product
 # forward (sb_lstm_fwd_args.products == 2) is the forward file again with -DSB_FWD_2P: its inference kernels only, launcher
 # sb_launch_lstm_fwd_bf_2p.
@@ -49,11 +59,11 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     os.makedirs(LIBDIR, exist_ok=True)
     objs, jobs = [], []
-    for src in SOURCES:
+    for src in SOURCES + SEQ_SOURCES:
         s = os.path.join(CSRC, src)
-        o = os.path.join(LIBDIR, src.replace(".hip", ".o"))
+        o = os.path.join(LIBDIR, os.path.basename(src).replace(".hip", ".o"))
         objs.append(o)
-        if force or _stale(o, [s] + HEADERS):
+        if force or _stale(o, [s] + (SEQ_HEADERS if src in SEQ_SOURCES else HEADERS)):
             cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-c", s, "-o", o]
             cmd[2:2] = os.environ.get("SB_EXTRA_HIPCC_FLAGS", "").split()     # e.g. -DSB_PHASE_TIMING (dev tool)
             cmd[2:2] = PER_FILE_FLAGS.get(src, [])

@@ -1077,3 +1077,6 @@ class MultiResoFuseLossFn(torch.autograd.Function):
     def backward(ctx, gout):
         (dest,) = ctx.saved_tensors
         return (dest * gout).view(ctx.shape), None, None
+
+
+from .functional_seq import GatedScanFn, LayerNormFn, gated_scan, gated_scan_step, layer_norm  # noqa: E402,F401

@@ -1,0 +1,78 @@
+"""Sequence-block operators with gradients: layer norm and the gated linear recurrence, beside the fused stages of functional.py.
+
+    u = layer_norm(x, w, b);  h, last = gated_scan(*proj(u).chunk(2, -1), h0)
+
+Any leading shape, float32 / bfloat16 / float16; the sums, statistics and states inside are float32.
+"""
+import torch
+
+from . import _lib as L
+from . import ops_seq
+
+
+class LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = ops_seq.layer_norm_fwd(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.wdtype = bias.dtype if bias is not None else None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        _, need_w, need_b, _ = ctx.needs_input_grad
+        dx, dw, db = ops_seq.layer_norm_bwd(dy, x, weight, mean, rstd, need_w, need_b, ctx.wdtype)
+        return dx if ctx.needs_input_grad[0] else None, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis, in x's type; weight / bias of shape (n,) in x's type or
+    float32"""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return LayerNormFn.apply(x, weight, bias, eps)
+    return ops_seq.layer_norm_fwd(x, weight, bias, eps, stats=False)[0]
+
+
+class GatedScanFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, h0, lengths, dim, form, reverse):
+        h, last, states = ops_seq.gated_scan_fwd(x, gate, h0, dim=dim, form=form, reverse=reverse, lengths=lengths)
+        ctx.save_for_backward(x, gate, states, lengths)
+        ctx.how = dict(dim=dim, form=form, reverse=reverse)
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dlast):
+        x, gate, states, lengths = ctx.saved_tensors
+        if dh is None and dlast is None:
+            return (None,) * 7
+        need = ctx.needs_input_grad
+        dx, dgate, dh0 = ops_seq.gated_scan_bwd(dh, dlast, x, gate, states, lengths=lengths, want_dh0=need[2], **ctx.how)
+        return dx if need[0] else None, dgate if need[1] else None, dh0, None, None, None, None
+
+
+def gated_scan(x, gate, h0=None, *, dim=1, form="sigmoid", reverse=False, lengths=None):
+    """-> (h, last): h_t = a_t h_{t-1} + b_t along axis `dim`; last (float32) is the state behind the last step.
+
+    form "sigmoid": a = sigmoid(gate), b = (1 - a) x; "decay": a = gate, b = x.  A chunk of up to 256 steps is joined by products of its
+    gates: with "decay" gates beyond 1 in magnitude, those products have to stay within float32.
+    h0: float32, x's shape without `dim` (None: zeros).  reverse: from the last step to the first.
+    lengths (int64 / int32, x.shape[:dim]): a padded batch; steps at and behind a sequence's length leave its state alone, their
+    outputs and gradients are 0 and their inputs are not looked at.
+    x and gate may be halves of one projection: a dense last axis is enough, other layouts are copied."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, h0)):
+        return GatedScanFn.apply(x, gate, h0, lengths, dim, form, reverse)
+    return ops_seq.gated_scan_fwd(x, gate, h0, dim=dim, form=form, reverse=reverse, lengths=lengths, save=False)[:2]
+
+
+def gated_scan_step(x, gate, state, *, form="sigmoid"):
+    """One step of gated_scan for streaming: state (float32, x's shape, dense) is updated in place; -> its value in x's type.  No
+    gradients: gated_scan with one step has them."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate, state)):
+        raise L.SoundBubbleHipError("gated_scan_step updates the state in place and has no gradient: call gated_scan, or this under "
+                                    "torch.no_grad()")
+    return ops_seq.gated_scan_step(x, gate, state, form=form)

@@ -2112,3 +2112,8 @@ def lstm_gen_bwd(dirs, rec, dhs, u, hs, geom, targets):
               dW2=t_wh, seg_len=geom.nsteps * geom.p_step, skip_first=geom.p_step if d == 0 else 0,
               skip_last=geom.p_step if d == 1 else 0, dbias=t_bi, dbias2=t_bh, gen_f16=True, gmax=gmax)
     return du
+
+
+# ---- sequence-block operators (include/sound_bubble_seq.h) ----
+from .ops_seq import (adamw_blocks, adamw_state, adamw_step, gated_scan_bwd, gated_scan_fwd, gated_scan_step,  # noqa: E402,F401
+                      layer_norm_bwd, layer_norm_fwd)

@@ -1,0 +1,380 @@
+"""Tensor-level wrappers of the sequence-block operators (include/sound_bubble_seq.h): layer norm, gated linear recurrence, AdamW
+over many tensors.
+
+float32, bfloat16 and float16 on a HIP device; anything else raises, there is no eager fallback.  The launches go to the current
+stream of the tensors' own device; what a call needs besides its results is allocated for the call.
+"""
+import ctypes as C
+import itertools
+import struct
+
+import torch
+
+from . import _lib as L
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+FORMS = {"decay": 0, "sigmoid": 1}
+
+
+def _fail(msg):
+    raise L.SoundBubbleHipError(msg)
+
+
+def _need(t, name, dtypes, device=None, shape=None):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
+        _fail(f"{name}: expected a tensor of {' / '.join(str(d)[6:] for d in dtypes)} on the GPU, got "
+              f"{type(t).__name__} {getattr(t, 'dtype', '')} {getattr(t, 'device', '')}")
+    if device is not None and t.device != device:
+        _fail(f"{name}: is on {t.device}, the call's tensors are on {device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        _fail(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class _On:
+    """the tensors' own device for the launches inside, and its current stream"""
+
+    def __init__(self, device):
+        self.ctx = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+        from . import ops
+        return ops._stream()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+        return False
+
+
+# ---- layer norm ----
+def _rows(t, n):
+    """-> (tensor, row stride): the last axis dense, all others one axis of rows; a copy where the strides do not allow that"""
+    if t.is_contiguous():
+        return t, n
+    t2 = t.reshape(-1, n)
+    if n > 1 and t2.stride(1) != 1:
+        t2 = t2.contiguous()
+    return t2, t2.stride(0) if t2.shape[0] > 1 else n
+
+
+def _norm_params(x, weight, bias):
+    if x.dim() < 1 or x.shape[-1] == 0:
+        _fail(f"layer_norm: x needs a last axis of at least one element, got shape {tuple(x.shape)}")
+    n = x.shape[-1]
+    for t, name in ((weight, "layer_norm: weight"), (bias, "layer_norm: bias")):
+        if t is not None:
+            _need(t, name, (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32), x.device, (n,))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        _fail(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
+    return n
+
+
+def layer_norm_fwd(x, weight, bias, eps=1e-5, stats=True):
+    """-> (y, mean, rstd): y = (x - mean) rstd weight + bias over the last axis, x's type; mean and rstd float32 of the leading
+    shape (None without `stats`).  weight / bias (None: 1 / 0) in x's type or float32."""
+    _need(x, "layer_norm: x", _TYPES)
+    n = _norm_params(x, weight, bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device).unbind(0)
+    rows = x.numel() // n
+    if rows == 0:
+        return y, mean, rstd
+    xr, ldx = _rows(x, n)
+    w, b = (t.contiguous() if t is not None else None for t in (weight, bias))
+    wt = w if w is not None else b
+    a = L.LayerNormArgs(rows, n, ldx, _TYPES[x.dtype], _TYPES[wt.dtype] if wt is not None else 0, eps, xr.data_ptr(), _ptr(w), _ptr(b),
+                        y.data_ptr(), _ptr(mean), _ptr(rstd))
+    with _On(x.device) as stream:
+        L.check(L.load().sb_layer_norm_fwd(a, stream), "sb_layer_norm_fwd")
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy, x, weight, mean, rstd, want_dw=True, want_db=True, wdtype=None):
+    """-> (dx, dw, db) of layer_norm_fwd; dw / db (None where not wanted) in `wdtype` (the weight's, or given for a bias alone),
+    summed over the rows in float32 in an order that the shape alone fixes"""
+    _need(x, "layer_norm_bwd: x", _TYPES)
+    n = _norm_params(x, weight, None)
+    _need(dy, "layer_norm_bwd: dy", (x.dtype,), x.device, x.shape)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if not _need(t, f"layer_norm_bwd: {name}", (torch.float32,), x.device, x.shape[:-1]).is_contiguous():
+            _fail(f"layer_norm_bwd: {name} must be contiguous")
+    wdtype = weight.dtype if weight is not None else (wdtype or x.dtype)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = torch.empty(n, dtype=wdtype, device=x.device) if want_dw else None
+    db = torch.empty(n, dtype=wdtype, device=x.device) if want_db else None
+    rows = x.numel() // n
+    xt = _TYPES[x.dtype]
+    lib = L.load()
+    scratch = None
+    if (want_dw or want_db) and rows:
+        scratch = torch.empty(lib.sb_layer_norm_bwd_scratch(rows, n, xt), dtype=torch.float32, device=x.device)
+    (xr, ldx), (dyr, lddy) = _rows(x, n), _rows(dy, n)
+    w = weight.contiguous() if weight is not None else None
+    a = L.LayerNormBwdArgs(rows, n, ldx, lddy, xt, _TYPES[wdtype], xr.data_ptr(), dyr.data_ptr(), _ptr(w), mean.data_ptr(), rstd.data_ptr(),
+                           dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(scratch))
+    if rows or want_dw or want_db:
+        with _On(x.device) as stream:
+            L.check(lib.sb_layer_norm_bwd(a, stream), "sb_layer_norm_bwd")
+    return dx, dw, db
+
+
+# ---- gated linear recurrence ----
+def _steps(t, outer, steps, inner):
+    """-> (tensor, outer stride, step stride) of the [outer, steps, inner] view with a dense inner axis; a copy where there is none"""
+    if t.is_contiguous():
+        return t, steps * inner, inner
+    t3 = t.reshape(outer, steps, inner)
+    if inner > 1 and t3.stride(2) != 1:
+        t3 = t3.contiguous()
+    return t3, t3.stride(0), t3.stride(1)
+
+
+def _scan_sizes(x, gate, dim, form, h0, lengths):
+    _need(x, "gated_scan: x", _TYPES)
+    _need(gate, "gated_scan: gate", (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32), x.device, x.shape)
+    if form not in FORMS:
+        _fail(f"gated_scan: form is one of {sorted(FORMS)}, got {form!r}")
+    if not (isinstance(dim, int) and 0 <= (dim if dim >= 0 else dim + x.dim()) < x.dim()):
+        _fail(f"gated_scan: dim {dim} is no axis of a tensor of shape {tuple(x.shape)}")
+    dim = dim % x.dim()
+    rest = x.shape[:dim] + x.shape[dim + 1:]
+    if h0 is not None:
+        _need(h0, "gated_scan: h0", (torch.float32,), x.device, rest)
+    if lengths is not None:
+        _need(lengths, "gated_scan: lengths", (torch.int64, torch.int32), x.device, x.shape[:dim])
+    outer = x.shape[:dim].numel()
+    return dim, rest, outer, x.shape[dim], x.shape[dim + 1:].numel()
+
+
+def _scan_plan(outer, steps, inner, xt):
+    got = [C.c_int64() for _ in range(3)]
+    L.check(L.load().sb_gated_scan_plan(outer, steps, inner, xt, *(C.byref(v) for v in got)), "sb_gated_scan_plan")
+    return [v.value for v in got]
+
+
+def gated_scan_fwd(x, gate, h0=None, *, dim=1, form="sigmoid", reverse=False, lengths=None, save=True):
+    """-> (h, h_last, states): h_t = a_t h_{t-1} + b_t along axis `dim`, from h0 (float32, x's shape without `dim`; None: zeros).
+    form "decay": a = gate, b = x; "sigmoid": a = sigmoid(gate), b = (1 - a) x.  h in x's type, h_last float32.
+    lengths (int64 / int32, x.shape[:dim]): steps behind a sequence's length leave its state alone and give 0.
+    states (None without `save`): what gated_scan_bwd needs, fp32."""
+    dim, rest, outer, steps, inner = _scan_sizes(x, gate, dim, form, h0, lengths)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.numel() == 0:
+        last = torch.zeros(rest, dtype=torch.float32, device=x.device) if h0 is None else h0.clone()
+        return h, last, torch.empty(0, dtype=torch.float32, device=x.device) if save else None
+    last = torch.empty(rest, dtype=torch.float32, device=x.device)
+    xt = _TYPES[x.dtype]
+    chunks, scratch_n, _ = _scan_plan(outer, steps, inner, xt)
+    states = torch.empty(chunks * outer * inner, dtype=torch.float32, device=x.device) if save else None
+    scratch = torch.empty(scratch_n, dtype=torch.float32, device=x.device) if scratch_n else None
+    x3, so_x, st_x = _steps(x, outer, steps, inner)
+    g3, so_g, st_g = _steps(gate, outer, steps, inner)
+    h0 = h0.contiguous() if h0 is not None else None
+    lengths = lengths.to(torch.int64).contiguous() if lengths is not None else None
+    a = L.GatedScanArgs(outer, steps, inner, xt, _TYPES[gate.dtype], FORMS[form], int(bool(reverse)), x3.data_ptr(), so_x, st_x,
+                        g3.data_ptr(), so_g, st_g, _ptr(h0), _ptr(lengths), h.data_ptr(), last.data_ptr(), _ptr(states), _ptr(scratch))
+    with _On(x.device) as stream:
+        L.check(L.load().sb_gated_scan_fwd(a, stream), "sb_gated_scan_fwd")
+    return h, last, states
+
+
+def gated_scan_bwd(dh, dlast, x, gate, states, *, dim=1, form="sigmoid", reverse=False, lengths=None, want_dh0=True):
+    """-> (dx, dgate, dh0): gradients of gated_scan_fwd's (h, h_last); dh / dlast None: zero.  `states` from gated_scan_fwd with the
+    same sizes.  dh0 float32 (None where not wanted)."""
+    dim, rest, outer, steps, inner = _scan_sizes(x, gate, dim, form, None, lengths)
+    if dh is not None:
+        _need(dh, "gated_scan_bwd: dh", (x.dtype,), x.device, x.shape)
+    if dlast is not None:
+        _need(dlast, "gated_scan_bwd: dlast", (torch.float32,), x.device, rest)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dgate = torch.empty(x.shape, dtype=gate.dtype, device=x.device)
+    if x.numel() == 0:
+        dh0 = None
+        if want_dh0:
+            dh0 = torch.zeros(rest, dtype=torch.float32, device=x.device) if dlast is None else dlast.clone()
+        return dx, dgate, dh0
+    xt = _TYPES[x.dtype]
+    chunks, _, scratch_n = _scan_plan(outer, steps, inner, xt)
+    _need(states, "gated_scan_bwd: states", (torch.float32,), x.device, (chunks * outer * inner,))
+    dh0 = torch.empty(rest, dtype=torch.float32, device=x.device) if want_dh0 else None
+    scratch = torch.empty(scratch_n, dtype=torch.float32, device=x.device) if scratch_n else None
+    x3, so_x, st_x = _steps(x, outer, steps, inner)
+    g3, so_g, st_g = _steps(gate, outer, steps, inner)
+    d3, so_d, st_d = _steps(dh, outer, steps, inner) if dh is not None else (None, 0, 0)
+    dlast = dlast.contiguous() if dlast is not None else None
+    lengths = lengths.to(torch.int64).contiguous() if lengths is not None else None
+    a = L.GatedScanBwdArgs(outer, steps, inner, xt, _TYPES[gate.dtype], FORMS[form], int(bool(reverse)), x3.data_ptr(), so_x, st_x,
+                           g3.data_ptr(), so_g, st_g, _ptr(d3), so_d, st_d, _ptr(dlast), _ptr(lengths), states.contiguous().data_ptr(),
+                           dx.data_ptr(), dgate.data_ptr(), _ptr(dh0), _ptr(scratch))
+    with _On(x.device) as stream:
+        L.check(L.load().sb_gated_scan_bwd(a, stream), "sb_gated_scan_bwd")
+    return dx, dgate, dh0
+
+
+def gated_scan_step(x, gate, state, *, form="sigmoid"):
+    """one step: `state` (float32, dense, x's shape) becomes a state + b in place -> its value in x's type"""
+    _need(x, "gated_scan_step: x", _TYPES)
+    _need(gate, "gated_scan_step: gate", (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32), x.device, x.shape)
+    _need(state, "gated_scan_step: state", (torch.float32,), x.device, x.shape)
+    if form not in FORMS:
+        _fail(f"gated_scan_step: form is one of {sorted(FORMS)}, got {form!r}")
+    if not state.is_contiguous():
+        _fail("gated_scan_step: state is updated in place and must be contiguous")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.numel() == 0:
+        return y
+    n = x.shape[-1] if x.dim() else 1
+    (xr, ldx), (gr, ldg) = _rows(x, n), _rows(gate, n)
+    with _On(x.device) as stream:
+        L.check(L.load().sb_gated_scan_step(xr.data_ptr(), gr.data_ptr(), state.data_ptr(), y.data_ptr(), x.numel() // n, n, ldx, ldg,
+                                            _TYPES[x.dtype], _TYPES[gate.dtype], FORMS[form], stream), "sb_gated_scan_step")
+    return y
+
+
+# ---- AdamW over many tensors ----
+def adamw_blocks(sizes):
+    """first block of each of the tensors in the state buffers, and behind the last one: a tensor starts at a multiple of
+    ADAMW_BLOCK elements"""
+    return list(itertools.accumulate(((n + L.ADAMW_BLOCK - 1) // L.ADAMW_BLOCK for n in sizes), initial=0))
+
+
+def adamw_state(params, bits=32):
+    """zero states for adamw_step: exp_avg, exp_avg_sq in one buffer each (float32, or float8_e4m3fn / float8_e5m2 codes with a
+    float8_e8m0fnu scale for every ADAMW_BLOCK elements), and `master`, float32, where a parameter has 16 bits"""
+    params = list(params)
+    if bits not in (32, 8):
+        _fail(f"adamw_state: bits is 32 or 8, got {bits}")
+    for p in params:
+        _need(p, "adamw_state: parameter", _TYPES, params[0].device)
+    starts = adamw_blocks([p.numel() for p in params])
+    blocks, dev = starts[-1], params[0].device if params else "cuda"
+    n = blocks * L.ADAMW_BLOCK
+    if bits == 32:
+        st = {k: torch.zeros(n, dtype=torch.float32, device=dev) for k in ("exp_avg", "exp_avg_sq")}
+    else:
+        st = {}
+        for k, t in (("exp_avg", torch.float8_e4m3fn), ("exp_avg_sq", torch.float8_e5m2)):
+            st[k] = torch.zeros(n, dtype=torch.uint8, device=dev).view(t)
+            st[k + "_scale"] = torch.zeros(blocks, dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu)
+    if any(p.dtype != torch.float32 for p in params):
+        st["master"] = torch.zeros(n, dtype=torch.float32, device=dev)
+        for p, b in zip(params, starts):
+            st["master"][b * L.ADAMW_BLOCK:b * L.ADAMW_BLOCK + p.numel()].copy_(p.detach().reshape(-1))
+    return st
+
+
+def _adamw_check_state(state, blocks, device, need_master):
+    n = blocks * L.ADAMW_BLOCK
+    eight = isinstance(state.get("exp_avg"), torch.Tensor) and state["exp_avg"].dtype == torch.float8_e4m3fn
+    want = {"exp_avg": (torch.float8_e4m3fn, n), "exp_avg_sq": (torch.float8_e5m2, n), "exp_avg_scale": (torch.float8_e8m0fnu, blocks),
+            "exp_avg_sq_scale": (torch.float8_e8m0fnu, blocks)} if eight else {k: (torch.float32, n) for k in ("exp_avg", "exp_avg_sq")}
+    if need_master:
+        want["master"] = (torch.float32, n)
+    for k, (t, size) in want.items():
+        b = _need(state.get(k), f"adamw_step: state[{k!r}]", (t,), device, (size,))
+        if not b.is_contiguous() or b.data_ptr() % 16:
+            _fail(f"adamw_step: state[{k!r}] must be contiguous and start at a multiple of 16 bytes")
+    return 8 if eight else 32
+
+
+def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, gscale=1.0, clip=0.0, seed=0,
+               skipped=None):
+    """One AdamW step (torch.optim.AdamW without amsgrad) over all tensors: `params` and `state` (adamw_state of the same
+    parameters) are updated in place.
+
+    grads: one a parameter, of its type or float32, None: that parameter and its states are left alone.
+    step: the step's number, from 1 on -- an int, or an int32 tensor of one element, which a captured graph reads at every replay.
+    lr: a number or a float32 tensor of one element.  clip > 0: the gradients, scaled by gscale, are clipped to that norm over all
+    tensors.  seed: of the 8-bit states' rounding.  skipped: counts a step that the device's watchdog word turned into a no-op
+    (ops.adam_step)."""
+    params, grads = list(params), list(grads)
+    if len(params) != len(grads):
+        _fail(f"adamw_step: {len(params)} parameters, {len(grads)} gradients")
+    if not params:
+        return
+    dev = params[0].device
+    sizes = [p.numel() for p in params]
+    starts = adamw_blocks(sizes)
+    need_master = False
+    groups = {}
+    for i, (p, g) in enumerate(zip(params, grads)):
+        t = p.dtype
+        if t not in _TYPES or not p.is_cuda or p.device != dev or not p.is_contiguous():
+            _fail(f"adamw_step: parameter {i}: expected a contiguous float32 / bfloat16 / float16 tensor on {dev}, got {t} on {p.device}"
+                  f"{'' if p.is_contiguous() else ', not contiguous'}")
+        need_master |= t != torch.float32
+        if g is None or sizes[i] == 0:
+            continue
+        gt = g.dtype
+        if (gt != t and gt != torch.float32) or g.device != dev or g.numel() != sizes[i] or g.shape != p.shape:
+            _fail(f"adamw_step: gradient {i}: expected {t} or float32 of shape {tuple(p.shape)} on {dev}, got {gt} {tuple(g.shape)} on {g.device}")
+        if not g.is_contiguous():
+            g = grads[i] = g.contiguous()
+        groups.setdefault((t, gt), []).append(i)
+    bits = _adamw_check_state(state, starts[-1], dev, need_master)
+    if starts[-1] >= 1 << 31:
+        _fail("adamw_step: more than 2^31 blocks of states")
+    step_dev = lr_dev = None
+    if isinstance(step, torch.Tensor):
+        step_dev, step = _need(step, "adamw_step: step", (torch.int32,), dev), 0
+        if step_dev.numel() != 1:
+            _fail("adamw_step: step is one number")
+    elif step < 1 or step >= 1 << 31:
+        _fail(f"adamw_step: step counts from 1, got {step}")
+    elif torch.cuda.is_current_stream_capturing():
+        _fail("adamw_step: a captured graph would repeat this step's number at every replay: pass step as an int32 tensor")
+    if isinstance(lr, torch.Tensor):
+        lr_dev, lr = _need(lr, "adamw_step: lr", (torch.float32,), dev), 0.0
+        if lr_dev.numel() != 1:
+            _fail("adamw_step: lr is one number")
+    if clip < 0:
+        _fail(f"adamw_step: clip is a norm (0: none), got {clip}")
+    lib = L.load()
+    chunk = lib.sb_adamw_chunk()
+    batches = [(key, ids[j:j + L.ADAMW_MAX]) for key, ids in groups.items() for j in range(0, len(ids), L.ADAMW_MAX)]
+    if not batches:
+        return
+    calls = []
+    for (t, gt), ids in batches:
+        a = L.AdamwArgs()
+        row, at = [], 0
+        for i in ids:
+            row += (params[i].data_ptr(), grads[i].data_ptr(), sizes[i], starts[i], at)
+            at += (sizes[i] + chunk - 1) // chunk
+        struct.pack_into("QQqii" * len(ids), a, 0, *row)
+        a.count, a.ptype, a.gtype, a.bits = len(ids), _TYPES[t], _TYPES[gt], bits
+        a.m, a.v = state["exp_avg"].data_ptr(), state["exp_avg_sq"].data_ptr()
+        if bits == 8:
+            a.m_scale, a.v_scale = state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()
+        if need_master:
+            a.master = state["master"].data_ptr()
+        a.lr, (a.beta1, a.beta2), a.eps, a.weight_decay = lr, betas, eps, weight_decay
+        a.lr_dev, a.step_dev, a.step, a.seed = _ptr(lr_dev), _ptr(step_dev), step, seed & 0xFFFFFFFF
+        a.gscale, a.clip = gscale, clip
+        calls.append(a)
+    calls[-1].last = 1
+    from . import ops
+    guard = ops._SCHED_STATUS.get(dev.index)
+    with _On(dev) as stream:
+        if clip > 0:
+            slots = L.ADAMW_NORM_SLOTS // len(calls)
+            if slots == 0:
+                _fail(f"adamw_step: clipping over more than {L.ADAMW_NORM_SLOTS * L.ADAMW_MAX} tensors")
+            part = torch.empty(L.ADAMW_NORM_SLOTS, dtype=torch.float64, device=dev)
+            for k, a in enumerate(calls):
+                L.check(lib.sb_adamw_norm(a, part.data_ptr(), k * slots, slots, stream), "sb_adamw_norm")
+        for a in calls:
+            if clip > 0:
+                a.norm_part, a.norm_slots = part.data_ptr(), slots * len(calls)
+            if guard is not None:
+                a.guard, a.skipped = guard.data_ptr(), _ptr(skipped)
+            L.check(lib.sb_adamw_step(a, stream), "sb_adamw_step")
