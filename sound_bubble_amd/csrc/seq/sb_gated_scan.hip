@@ -1,10 +1,11 @@
 // Gated linear recurrence over the middle axis of [outer, steps, inner]:  h_t = a_t h_{t-1} + b_t, forward, backward, one step.
 //
-// Steps are joined as pairs (A, B): h -> A h + B; (A2, B2) after (A1, B1) is (A2 A1, A2 B1 + B2).  A thread holds V channels of S
-// consecutive steps in registers and joins them in order; the threads along time are joined over lanes (distances 1, 2, 4, ...),
-// waves through LDS, and the state is carried from chunk to chunk by the same workgroup, so x and gate are read once and the
-// order of all products is fixed by the sizes.  Where there are too few columns (sequence x channel tile) to fill the chip, time is
-// cut into segments: a first kernel makes each segment's pair, the second joins those in front of its own.
+// Steps are joined as pairs (A, B): h -> A h + B; (A2, B2) after (A1, B1) is (A2 A1, A2 B1 + B2).  A lane holds one channel of one
+// sequence, S consecutive steps of it in registers, and all lanes of a wave are at the same steps, so that a step's address and what
+// is live are the wave's business and nothing goes over lanes.  The waves of a workgroup are consecutive in time; their pairs meet
+// in LDS, where every wave joins them in the same order, and the state is carried from chunk to chunk by the same workgroup: x and gate
+// are read once and the order of all products is fixed by the sizes.  Where there are too few channels to fill the chip, time is cut
+// into segments: a first kernel makes each segment's pair, the second joins those in front of its own.
 // Steps that a sequence does not have (behind its length, behind the last chunk) are (1, 0) by selection, whatever memory holds.
 //
 // The backward pass makes h_{t-1} again in fp32 from the states the forward pass left in front of every chunk, and walks
@@ -14,52 +15,36 @@
 
 namespace {
 
-constexpr int S = 8;               // steps a thread holds
-constexpr int kMaxSplits = 64;
+// Steps a lane holds, and waves of a workgroup (which then has 256 registers a lane).  bf16 8 x 4096 x 2048, forward / backward, us: 16 x 8
+// 98 / 160, 8 x 16 108 / 176, 8 x 8 111 / 162; two channels a lane: 179 / 250 (half the workgroups, twice the registers).
+constexpr int S = 16, kMaxWaves = 8;
+// Workgroups with fewer waves than kFewWaves in all leave the chip half empty: time is cut so that there are about kWaves.  That reads x and
+// gate twice.  fp16 6 x 3001 x 1000 (752 waves) forward / backward, us: cut 68 / 94, whole 94 / 134.
+constexpr int kFewWaves = 1024, kWaves = 4096, kMaxSplits = 64;
 
-// how a wave is laid over a column: lane = (column of the wave, segment, channel vector)
 struct Lay {
-  int lc, lseg, nw;                // lanes along channels, lanes along time, waves along time (powers of two)
-  int64_t tiles, cols;             // channel tiles of a sequence, columns
-  int per;                         // columns of a workgroup
-  int64_t steps;                   // steps of a chunk
-  int64_t groups() const { return (cols + per - 1) / per; }
+  int nw, splits;                  // waves along time, segments of time
+  int64_t tiles;                   // workgroups' channel tiles: 64 lanes of the flattened (sequence, channel) axis
+  int64_t steps, chunks;           // steps of a chunk, chunks of a sequence
 };
 
-int pow2_up(int64_t v, int most) {
-  int p = 1;
-  while (p < most && p < v) p *= 2;
-  return p;
-}
-
-Lay lay_of(int64_t outer, int64_t steps, int64_t inner, int V, int full_lc) {
+Lay lay_of(int64_t outer, int64_t steps, int64_t inner) {
   Lay l;
-  l.lc = pow2_up((inner + V - 1) / V, full_lc);
-  l.lseg = pow2_up((steps + S - 1) / S, 64 / l.lc);
-  l.tiles = (inner + l.lc * V - 1) / (l.lc * V);
-  l.cols = outer * l.tiles;
-  l.per = 64 / (l.lc * l.lseg);
-  l.nw = l.per == 1 && steps > (int64_t)l.lseg * S && l.cols < 2048 ? 4 : 1;
-  l.steps = (int64_t)l.lseg * l.nw * S;
+  l.tiles = (outer * inner + 63) / 64;
+  l.nw = 1;
+  // (more waves along time until there are 8 a SIMD: fp32 16 x 625 x 4640 forward 115 us, with half as many 123)
+  while (l.nw < kMaxWaves && l.nw * S < steps && l.tiles * l.nw < 8192) l.nw *= 2;
+  l.steps = (int64_t)l.nw * S;
+  l.chunks = (steps + l.steps - 1) / l.steps;
+  l.splits = 1;
+  const int64_t waves = l.tiles * l.nw;
+  if (waves < kFewWaves && l.chunks >= 4) l.splits = (int)std::min<int64_t>(std::min<int64_t>(kMaxSplits, l.chunks / 2), (kWaves + waves - 1) / waves);
   return l;
 }
 
-// channels of a thread and lanes along channels: 128 bytes of a step's row
-int fwd_vec(int64_t inner, int xtype) { return xtype == SB_F32 ? (inner < 4 ? 1 : 4) : (inner < 8 ? 1 : 8); }
-int bwd_vec(int64_t inner) { return inner < 4 ? 1 : 4; }
-Lay fwd_lay(int64_t outer, int64_t steps, int64_t inner, int xtype) { return lay_of(outer, steps, inner, fwd_vec(inner, xtype), 8); }
-Lay bwd_lay(int64_t outer, int64_t steps, int64_t inner, int xtype) { return lay_of(outer, steps, inner, bwd_vec(inner), xtype == SB_F32 ? 8 : 16); }
-
-int splits_of(const Lay& l, int64_t steps) {
-  const int64_t chunks = (steps + l.steps - 1) / l.steps, waves = l.groups() * l.nw;
-  if (waves >= 1024 || chunks < 4) return 1;
-  return (int)std::min<int64_t>(std::min<int64_t>(kMaxSplits, chunks / 2), (2048 + waves - 1) / waves);
-}
-
 struct Kargs {
-  int64_t outer, steps, inner, tiles, cols, keep;      // keep: steps between two kept states
-  int lc, lseg, reverse, splits;
-  int64_t chunks, chunk_steps;
+  int64_t outer, steps, inner, chunks, chunk_steps;
+  int reverse, splits;
   const void* x; int64_t so_x, st_x;
   const void* gate; int64_t so_g, st_g;
   const void* dh; int64_t so_d, st_d;
@@ -82,414 +67,344 @@ SB_DEVINL void logistic(float z, float& a, float& one_less) {
   one_less = pos ? q : r;
 }
 
-// Where a thread stands.  A sequence whose channels do not fill its last tile's vectors has that tile's vectors moved back to end
-// with the last channel: two threads then make the same channels, to the same bits, and no vector is cut (V = 1 where inner < V).
-template <int V> struct Place {
-  int lane, wave, lc, seg, tseg;
-  bool on;                                // the thread has channels
-  int64_t o, c, lo, hi;                   // sequence, first channel, live steps [lo, hi) in the order of the walk
-  bool all;                               // every thread of the workgroup has
+// where a lane stands
+struct Place {
+  int wave, waves;
+  bool on;                                // the lane has a channel
+  int64_t q, o, c, lo, hi;                // flattened channel, sequence, channel, live steps [lo, hi) in the order of the walk
+  int64_t all_lo, all_hi;                 // steps that are live in every lane of the wave (uniform)
   SB_DEVINL Place(const Kargs& k) {
-    lane = threadIdx.x & 63;
-    wave = threadIdx.x >> 6;
-    lc = lane & (k.lc - 1);
-    seg = (lane / k.lc) & (k.lseg - 1);
-    tseg = wave * k.lseg + seg;
-    const int per = 64 / (k.lc * k.lseg);
-    const int64_t col = (int64_t)blockIdx.x * per + lane / (k.lc * k.lseg);
-    o = col / k.tiles;
-    c = (col - o * k.tiles) * (k.lc * V) + lc * V;
-    on = col < k.cols && c < k.inner;
-    int64_t n = 0;
-    if (on) {
-      c = min(c, k.inner - V);
-      n = k.len ? min(max(k.len[o], (int64_t)0), k.steps) : k.steps;
-    } else {
-      o = c = 0;
-    }
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    waves = blockDim.x >> 6;
+    q = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63));
+    on = q < k.outer * k.inner;
+    o = on ? q / k.inner : 0;
+    c = on ? q - o * k.inner : 0;
+    q = on ? q : 0;
+    int64_t n = on ? k.steps : 0;
+    if (on && k.len) n = min(max(k.len[o], (int64_t)0), k.steps);
     lo = k.reverse ? k.steps - n : 0;
     hi = k.reverse ? k.steps : n;
-    all = __syncthreads_and(on) != 0;
+    all_lo = lo;
+    all_hi = hi;
+    if (!__all(on && n == k.steps)) {
+      for (int d = 1; d < 64; d *= 2) {
+        all_lo = max(all_lo, (int64_t)__shfl_xor((long long)all_lo, d, 64));
+        all_hi = min(all_hi, (int64_t)__shfl_xor((long long)all_hi, d, 64));
+      }
+    }
+    all_lo = first(all_lo);
+    all_hi = __all(on) ? first(all_hi) : 0;
   }
-  // live steps of the thread's S from `first` on, as a bit each
-  SB_DEVINL unsigned live(int64_t first) const {
-    const int n0 = (int)min(max(lo - first, (int64_t)0), (int64_t)S), n1 = (int)min(max(hi - first, (int64_t)0), (int64_t)S);
+  static SB_DEVINL int64_t first(int64_t v) {
+    return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+  }
+  // live steps of the lane's S from t on, as a bit each
+  SB_DEVINL unsigned live(int64_t t) const {
+    const int n0 = (int)min(max(lo - t, (int64_t)0), (int64_t)S), n1 = (int)min(max(hi - t, (int64_t)0), (int64_t)S);
     return ((1u << n1) - 1u) & ~((1u << n0) - 1u);
+  }
+  SB_DEVINL bool full(int64_t t) const { return t >= all_lo && t + S <= all_hi; }
+};
+
+template <class E> SB_DEVINL void load_steps(E (&v)[S], const void* base, int64_t so, int64_t st, const Place& p, const Kargs& k, int64_t t, bool full,
+                                             unsigned live) {
+  const int64_t step = k.reverse ? -st : st;
+  const E* at = (const E*)base + (k.reverse ? k.steps - 1 - t : t) * st + p.o * so + p.c;
+  if (full) {
+#pragma unroll
+    for (int s = 0; s < S; ++s, at += step) v[s] = *at;
+  } else {
+#pragma unroll
+    for (int s = 0; s < S; ++s, at += step) {
+      v[s] = (E)0.f;
+      if (live >> s & 1) v[s] = *at;
+    }
+  }
+}
+template <class E> SB_DEVINL void store_steps(void* base, const E (&v)[S], const Place& p, const Kargs& k, int64_t t, bool full) {
+  const int64_t step = k.reverse ? -k.inner : k.inner;
+  E* at = (E*)base + ((k.reverse ? k.steps - 1 - t : t) + p.o * k.steps) * k.inner + p.c;
+  if (full) {
+#pragma unroll
+    for (int s = 0; s < S; ++s, at += step) *at = v[s];
+  } else if (p.on) {
+#pragma unroll
+    for (int s = 0; s < S; ++s, at += step)
+      if (t + s < k.steps) *at = v[s];
+  }
+}
+
+// Everything this wave has under way has arrived.  In front of a loop whose loads wait by count for one round: without it the counts
+// have to allow for what was issued on the way in, and the loop would wait for its own stores.
+SB_DEVINL void wait_memory() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);      // vmcnt(0)
+}
+// a barrier that leaves loads and stores under way: the waves exchange nothing but LDS
+SB_DEVINL void block_sync() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);      // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// a_t and what multiplies x_t
+template <int FORM> SB_DEVINL void coefficients(float g, float& a, float& ol) {
+  if constexpr (FORM == SB_SCAN_SIGMOID) {
+    logistic(g, a, ol);
+  } else {
+    a = g;
+    ol = 1.f;
+  }
+}
+SB_DEVINL void kill_dead(float (&a)[S], float (&ol)[S], unsigned live) {
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    a[s] = live >> s & 1 ? a[s] : 1.f;
+    ol[s] = live >> s & 1 ? ol[s] : 0.f;
+  }
+}
+template <class E> SB_DEVINL void kill_dead(E (&v)[S], unsigned live) {
+#pragma unroll
+  for (int s = 0; s < S; ++s) v[s] = live >> s & 1 ? v[s] : (E)0.f;
+}
+
+// the pairs of a workgroup's waves, two buffers in turn: [turn][wave][lane]
+struct Pairs {
+  float2* lds;
+  int waves;
+  SB_DEVINL float2& at(int turn, int wave) const { return lds[(turn * waves + wave) * 64 + (threadIdx.x & 63)]; }
+  // carry over all waves; in: what enters wave `mine`
+  template <bool UP> SB_DEVINL void join(int turn, int mine, float& carry, float& in) const {
+    for (int w = 0; w < waves; ++w) {
+      const int j = UP ? w : waves - 1 - w;
+      const float2 r = at(turn, j);
+      if (j == mine) in = carry;
+      carry = __builtin_fmaf(r.x, carry, r.y);
+    }
+  }
+  SB_DEVINL float product(int turn) const {
+    float v = 1.f;
+    for (int w = 0; w < waves; ++w) v *= at(turn, w).x;
+    return v;
   }
 };
 
-template <class E, int V> SB_DEVINL void load_steps(Vec<E, V> (&v)[S], const void* base, int64_t so, int64_t st, const Place<V>& p, const Kargs& k,
-                                                    int64_t t0, bool full) {
-  const int64_t first = t0 + (int64_t)p.tseg * S;
-  const int64_t step = k.reverse ? -st : st;
-  const E* at = (const E*)base + p.o * so + p.c + (k.reverse ? k.steps - 1 - first : first) * st;
-  if (full) {
+// state in front of segment `split`: h0 and the pairs of the earlier ones (UP), dlast and those of the later ones (!UP)
+template <bool UP> SB_DEVINL float fold_splits(const float* start, const Place& p, const Kargs& k, int split) {
+  const int64_t plane = k.outer * k.inner;
+  if (!p.on) return 0.f;
+  float carry = start ? start[p.q] : 0.f;
+  const int n = UP ? split : k.splits - 1 - split;
+  constexpr int N = 16;
+  for (int j0 = 0; j0 < n; j0 += N) {      // (the loads of N pairs at once: one after the other they cost a trip to memory each)
+    float A[N], B[N];
 #pragma unroll
-    for (int s = 0; s < S; ++s) v[s] = vload<E, V>(at + s * step);
-  } else {
-    const unsigned live = p.live(first);
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[s].v[i] = (E)0.f;
-      if (live >> s & 1) v[s] = vload<E, V>(at + s * step);
+    for (int i = 0; i < N; ++i) {
+      const int j = UP ? j0 + i : k.splits - 1 - j0 - i;
+      A[i] = j0 + i < n ? k.agg[(2 * j) * plane + p.q] : 1.f;
+      B[i] = j0 + i < n ? k.agg[(2 * j + 1) * plane + p.q] : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (j0 + i < n) carry = __builtin_fmaf(A[i], carry, B[i]);
   }
-}
-
-template <class E, int V> SB_DEVINL void store_steps(void* base, const Vec<E, V> (&v)[S], const Place<V>& p, const Kargs& k, int64_t t0, bool full) {
-  const int64_t first = t0 + (int64_t)p.tseg * S;
-  const int64_t step = k.reverse ? -k.inner : k.inner;
-  E* at = (E*)base + (p.o * k.steps + (k.reverse ? k.steps - 1 - first : first)) * k.inner + p.c;
-  if (full) {
-#pragma unroll
-    for (int s = 0; s < S; ++s) vstore<E, V>(at + s * step, v[s]);
-  } else if (p.on) {
-    const int n = (int)min(max(k.steps - first, (int64_t)0), (int64_t)S);
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-      if (s < n) vstore<E, V>(at + s * step, v[s]);
-  }
-}
-
-// lanes' pairs, in place, to the pair of all segments in front of (UP) / behind (!UP) the thread's own within its wave; -> the wave's whole in tot
-template <bool UP, int V> SB_DEVINL void join_lanes(float (&A)[V], float (&B)[V], const Place<V>& p, const Kargs& k, float (&tA)[V], float (&tB)[V]) {
-  for (int d = 1; d < k.lseg; d *= 2) {
-    const int from = UP ? p.lane - d * k.lc : p.lane + d * k.lc;
-    const bool has = UP ? p.seg >= d : p.seg + d < k.lseg;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float a = __shfl(A[i], from & 63, 64), b = __shfl(B[i], from & 63, 64);
-      if (has) {
-        B[i] = __builtin_fmaf(A[i], b, B[i]);
-        A[i] *= a;
-      }
-    }
-  }
-  const int base = p.lane - p.seg * k.lc;
-  const int end = UP ? base + (k.lseg - 1) * k.lc : base, from = UP ? p.lane - k.lc : p.lane + k.lc;
-  const bool has = UP ? p.seg > 0 : p.seg < k.lseg - 1;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    tA[i] = __shfl(A[i], end, 64);
-    tB[i] = __shfl(B[i], end, 64);
-    const float a = __shfl(A[i], from & 63, 64), b = __shfl(B[i], from & 63, 64);
-    A[i] = has ? a : 1.f;
-    B[i] = has ? b : 0.f;
-  }
-}
-
-// carry over the waves: `in` = what enters the thread's wave, `carry` = what leaves the workgroup's chunk
-template <bool UP, int V, int NW> SB_DEVINL void join_waves(float (*lds)[16 * V][2], const float (&tA)[V], const float (&tB)[V], const Place<V>& p,
-                                                            float (&carry)[V], float (&in)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) in[i] = carry[i];
-  if constexpr (NW == 1) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = __builtin_fmaf(tA[i], carry[i], tB[i]);
-  } else {
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const int j = UP ? w : NW - 1 - w;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (j == p.wave) in[i] = carry[i];
-        carry[i] = __builtin_fmaf(lds[j][p.lc * V + i][0], carry[i], lds[j][p.lc * V + i][1]);
-      }
-    }
-  }
-}
-template <int V> SB_DEVINL void put_waves(float (*lds)[16 * V][2], const float (&tA)[V], const float (&tB)[V], const Place<V>& p) {
-  if (p.seg == 0) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      lds[p.wave][p.lc * V + i][0] = tA[i];
-      lds[p.wave][p.lc * V + i][1] = tB[i];
-    }
-  }
-}
-
-template <class G, int FORM, int V> SB_DEVINL void coefficients(const Vec<G, V>& g, float (&a)[V], float (&one_less)[V], bool live) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if constexpr (FORM == SB_SCAN_SIGMOID)
-      logistic((float)g.v[i], a[i], one_less[i]);
-    else {
-      a[i] = (float)g.v[i];
-      one_less[i] = 1.f;
-    }
-    if (!live) {
-      a[i] = 1.f;
-      one_less[i] = 0.f;
-    }
-  }
-}
-
-// state in front of split `split`: h0 and the pairs of the earlier ones (UP), dlast and those of the later ones (!UP)
-template <bool UP, int V> SB_DEVINL void fold_splits(float (&carry)[V], const float* start, const Place<V>& p, const Kargs& k, int split) {
-  const int64_t oc = p.o * k.inner + p.c, plane = k.outer * k.inner;
-#pragma unroll
-  for (int i = 0; i < V; ++i) carry[i] = 0.f;
-  if (!p.on) return;
-  if (start) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = start[oc + i];
-  }
-  for (int j = UP ? 0 : k.splits - 1; UP ? j < split : j > split; j += UP ? 1 : -1) {
-    const Vec<float, V> A = vload<float, V>(k.agg + (2 * j) * plane + oc), B = vload<float, V>(k.agg + (2 * j + 1) * plane + oc);
-#pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = __builtin_fmaf(A.v[i], carry[i], B.v[i]);
-  }
+  return carry;
 }
 
 // MODE 0: h, states, h_last.  MODE 1: the pair of segment blockIdx.y into agg.
-template <class T, class G, int FORM, int V, int NW, int MODE>
-__global__ __launch_bounds__(64 * NW) void gated_scan_fwd_kernel(Kargs k) {
-  __shared__ float lds[2][NW][16 * V][2];
-  const Place<V> p(k);
+template <class T, class G, int FORM, int MODE>
+__global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(Kargs k) {
+  extern __shared__ float2 lds[];
+  const Place p(k);
+  const Pairs pairs{lds, p.waves};
   const int split = blockIdx.y;
-  const int64_t c0 = k.chunks * split / k.splits, c1 = k.chunks * (split + 1) / k.splits;
-  float carry[V], whole[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    carry[i] = 0.f;
-    whole[i] = 1.f;
-  }
-  if constexpr (MODE == 0) fold_splits<true, V>(carry, k.h0, p, k, split);
-  Vec<T, V> x[S];
-  Vec<G, V> g[S];
-  const auto is_full = [&](int64_t chunk) {
-    const int64_t t0 = chunk * k.chunk_steps;
-    return p.all && !k.len && t0 + k.chunk_steps <= k.steps;
+  const int64_t c0 = k.chunks * split / k.splits, c1 = k.chunks * (split + 1) / k.splits, plane = k.outer * k.inner;
+  float carry = MODE == 0 ? fold_splits<true>(k.h0, p, k, split) : 0.f, whole = 1.f;
+  T x[S];
+  G g[S];
+  const auto load = [&](int64_t t, bool full) __attribute__((always_inline)) {
+    const unsigned live = full ? 0u : p.live(t);
+    load_steps<T>(x, k.x, k.so_x, k.st_x, p, k, t, full, live);
+    load_steps<G>(g, k.gate, k.so_g, k.st_g, p, k, t, full, live);
   };
-  load_steps<T, V>(x, k.x, k.so_x, k.st_x, p, k, c0 * k.chunk_steps, is_full(c0));
-  load_steps<G, V>(g, k.gate, k.so_g, k.st_g, p, k, c0 * k.chunk_steps, is_full(c0));
-  for (int64_t ch = c0; ch < c1; ++ch) {
-    const int64_t t0 = ch * k.chunk_steps, first = t0 + (int64_t)p.tseg * S;
-    const bool full = is_full(ch);
-    const unsigned live = p.live(first);
-    float a[S][V], b[S][V], A[V], B[V];
+  const auto start = [&](int64_t ch) { return ch * k.chunk_steps + p.wave * S; };
+  // FAST: this chunk and the next have all their steps in this wave
+  const auto chunk = [&](int64_t ch, auto fast) __attribute__((always_inline)) {
+    constexpr bool FAST = decltype(fast)::value;
+    const int64_t t = start(ch);
+    const bool full = FAST || p.full(t);
+    const unsigned live = full ? 0u : p.live(t);
+    float a[S], b[S], xf[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      coefficients<G, FORM, V>(g[s], a[s], b[s], full || (live >> s & 1));
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        b[s][i] *= (float)x[s].v[i];
-        A[i] = s ? A[i] * a[s][i] : a[s][i];
-        B[i] = s ? __builtin_fmaf(a[s][i], B[i], b[s][i]) : b[s][i];
-      }
+      xf[s] = (float)x[s];
+      a[s] = (float)g[s];
     }
-    if (ch + 1 < c1) {
-      load_steps<T, V>(x, k.x, k.so_x, k.st_x, p, k, t0 + k.chunk_steps, is_full(ch + 1));
-      load_steps<G, V>(g, k.gate, k.so_g, k.st_g, p, k, t0 + k.chunk_steps, is_full(ch + 1));
-    }
-    float tA[V], tB[V], in[V];
-    join_lanes<true, V>(A, B, p, k, tA, tB);
-    if constexpr (NW > 1) {
-      put_waves<V>(lds[ch & 1], tA, tB, p);
-      __syncthreads();
-    }
-    if constexpr (MODE == 1) {
-      if constexpr (NW == 1) {
+    if constexpr (FAST) load(t + k.chunk_steps, true);
+    else if (ch + 1 < c1) load(t + k.chunk_steps, p.full(t + k.chunk_steps));
 #pragma unroll
-        for (int i = 0; i < V; ++i) whole[i] *= tA[i];
-      } else {
+    for (int s = 0; s < S; ++s) coefficients<FORM>(a[s], a[s], b[s]);
+    if (!full) kill_dead(a, b, live);
+    float A, B;
 #pragma unroll
-        for (int w = 0; w < NW; ++w)
-#pragma unroll
-          for (int i = 0; i < V; ++i) whole[i] *= lds[ch & 1][w][p.lc * V + i][0];
-      }
+    for (int s = 0; s < S; ++s) {
+      b[s] *= xf[s];      // (dead steps were loaded as 0)
+      A = s ? A * a[s] : a[s];
+      B = s ? __builtin_fmaf(a[s], B, b[s]) : b[s];
     }
-    join_waves<true, V, NW>(lds[ch & 1], tA, tB, p, carry, in);
+    if (MODE == 0 && k.states && p.wave == 0 && p.on) k.states[ch * plane + p.q] = carry;
+    float in;
+    if (p.waves > 1) {
+      pairs.at(ch & 1, p.wave) = make_float2(A, B);
+      block_sync();
+      if constexpr (MODE == 1) whole *= pairs.product(ch & 1);
+      pairs.template join<true>(ch & 1, p.wave, carry, in);
+    } else {
+      in = carry;
+      carry = __builtin_fmaf(A, carry, B);
+      if constexpr (MODE == 1) whole *= A;
+    }
     if constexpr (MODE == 0) {
-      float h[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[i] = __builtin_fmaf(A[i], in[i], B[i]);
-      if (k.states && p.on && (first & (k.keep - 1)) == 0 && first < k.steps) {
-        Vec<float, V> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = h[i];
-        vstore<float, V>(k.states + (first / k.keep) * (k.outer * k.inner) + p.o * k.inner + p.c, o);
-      }
-      Vec<T, V> out[S];
+      T out[S];
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const bool lives = full || (live >> s & 1);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          h[i] = __builtin_fmaf(a[s][i], h[i], b[s][i]);
-          out[s].v[i] = lives ? (T)h[i] : (T)0.f;
-        }
+        in = __builtin_fmaf(a[s], in, b[s]);
+        out[s] = (T)in;
       }
-      store_steps<T, V>(k.h, out, p, k, t0, full);
+      if (!full) kill_dead<T>(out, live);
+      store_steps<T>(k.h, out, p, k, t, full);
     }
+  };
+  load(start(c0), p.full(start(c0)));
+  for (int64_t ch = c0; ch < c1; ++ch) {
+    wait_memory();
+    for (; ch + 1 < c1 && p.full(start(ch)) && p.full(start(ch + 1)); ++ch) chunk(ch, std::true_type());
+    chunk(ch, std::false_type());
   }
-  if (p.tseg == 0 && p.on) {
-    const int64_t oc = p.o * k.inner + p.c;
-    Vec<float, V> o, w;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      o.v[i] = carry[i];
-      w.v[i] = whole[i];
-    }
+  if (p.wave == 0 && p.on) {
     if constexpr (MODE == 0) {
-      if (split == k.splits - 1) vstore<float, V>(k.h_last + oc, o);
+      if (split == k.splits - 1) k.h_last[p.q] = carry;
     } else {
-      const int64_t plane = k.outer * k.inner;
-      vstore<float, V>(k.agg + (2 * split) * plane + oc, w);
-      vstore<float, V>(k.agg + (2 * split + 1) * plane + oc, o);
+      k.agg[(2 * split) * plane + p.q] = whole;
+      k.agg[(2 * split + 1) * plane + p.q] = carry;
     }
   }
 }
 
 // MODE 0: dx, dgate, dh0.  MODE 1: the pair (A, D) of segment blockIdx.y + 1 into agg.
-template <class T, class G, int FORM, int V, int NW, int MODE>
-__global__ __launch_bounds__(64 * NW) void gated_scan_bwd_kernel(Kargs k) {
-  __shared__ float lds[2][2][NW][16 * V][2];
-  const Place<V> p(k);
+template <class T, class G, int FORM, int MODE>
+__global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(Kargs k) {
+  extern __shared__ float2 lds[];
+  const Place p(k);
+  const Pairs down{lds, p.waves}, up{lds + 2 * 64 * p.waves, p.waves};
   const int split = blockIdx.y + (MODE == 1 ? 1 : 0);
-  const int64_t c0 = k.chunks * split / k.splits, c1 = k.chunks * (split + 1) / k.splits;
-  const int64_t oc = p.o * k.inner + p.c, plane = k.outer * k.inner;
-  float carry[V], whole[V];
+  const int64_t c0 = k.chunks * split / k.splits, c1 = k.chunks * (split + 1) / k.splits, plane = k.outer * k.inner;
+  float carry = MODE == 0 ? fold_splits<false>(k.dlast, p, k, split) : 0.f, whole = 1.f;
+  T x[S], d[S];
+  G g[S];
+  float state = 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    carry[i] = 0.f;
-    whole[i] = 1.f;
-  }
-  if constexpr (MODE == 0) fold_splits<false, V>(carry, k.dlast, p, k, split);
-  Vec<T, V> x[S], d[S];
-  Vec<G, V> g[S];
-  Vec<float, V> state;
-  const auto is_full = [&](int64_t chunk) {
-    const int64_t t0 = chunk * k.chunk_steps;
-    return p.all && !k.len && t0 + k.chunk_steps <= k.steps;
-  };
-  const auto load = [&](int64_t ch) __attribute__((always_inline)) {
-    const int64_t t0 = ch * k.chunk_steps;
-    const bool full = is_full(ch);
-    load_steps<G, V>(g, k.gate, k.so_g, k.st_g, p, k, t0, full);
-    if (k.dh) load_steps<T, V>(d, k.dh, k.so_d, k.st_d, p, k, t0, full);
+  for (int s = 0; s < S; ++s) d[s] = (T)0.f;
+  const auto load = [&](int64_t ch, int64_t t, bool full, bool has) __attribute__((always_inline)) {
+    const unsigned live = full ? 0u : p.live(t);
+    load_steps<G>(g, k.gate, k.so_g, k.st_g, p, k, t, full, live);
+    if (has) load_steps<T>(d, k.dh, k.so_d, k.st_d, p, k, t, full, live);
     if constexpr (MODE == 0) {
-      load_steps<T, V>(x, k.x, k.so_x, k.st_x, p, k, t0, full);
-      if (p.on) state = vload<float, V>(k.states + ch * plane + oc);
+      load_steps<T>(x, k.x, k.so_x, k.st_x, p, k, t, full, live);
+      if (p.on) state = k.states[ch * plane + p.q];
     }
   };
-#pragma unroll
-  for (int s = 0; s < S; ++s)
-#pragma unroll
-    for (int i = 0; i < V; ++i) d[s].v[i] = (T)0.f;
-#pragma unroll
-  for (int i = 0; i < V; ++i) state.v[i] = 0.f;
-  load(c1 - 1);
-  for (int64_t ch = c1 - 1; ch >= c0; --ch) {
-    const int64_t t0 = ch * k.chunk_steps, first = t0 + (int64_t)p.tseg * S;
-    const bool full = is_full(ch);
-    const unsigned live = p.live(first);
-    float a[S][V], ol[S][V], A[V], D[V];
-    float xf[S][V], df[S][V];
+  const auto start = [&](int64_t ch) { return ch * k.chunk_steps + p.wave * S; };
+  const auto chunk = [&](int64_t ch, auto fast) __attribute__((always_inline)) {
+    constexpr bool FAST = decltype(fast)::value;
+    const int64_t t = start(ch);
+    const bool full = FAST || p.full(t);
+    const unsigned live = full ? 0u : p.live(t);
+    float a[S], ol[S], xf[S], df[S], h = state;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const bool lives = full || (live >> s & 1);
-      coefficients<G, FORM, V>(g[s], a[s], ol[s], lives);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        xf[s][i] = MODE == 0 ? (float)x[s].v[i] : 0.f;      // (dead steps were loaded as 0)
-        df[s][i] = (float)d[s].v[i];
-      }
+      a[s] = (float)g[s];
+      xf[s] = MODE == 0 ? (float)x[s] : 0.f;      // (dead steps were loaded as 0)
+      df[s] = (float)d[s];
     }
+    if constexpr (FAST) load(ch - 1, t - k.chunk_steps, true, true);
+    else if (ch > c0) load(ch - 1, t - k.chunk_steps, p.full(t - k.chunk_steps), k.dh != nullptr);
 #pragma unroll
-    for (int s = S - 1; s >= 0; --s)
+    for (int s = 0; s < S; ++s) coefficients<FORM>(a[s], a[s], ol[s]);
+    if (!full) kill_dead(a, ol, live);
+    float A, D, B;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        A[i] = s < S - 1 ? A[i] * a[s][i] : a[s][i];
-        D[i] = a[s][i] * (s < S - 1 ? df[s][i] + D[i] : df[s][i]);
-      }
-    float fA[V], fB[V], fin[V];
+    for (int s = S - 1; s >= 0; --s) {
+      A = s < S - 1 ? A * a[s] : a[s];
+      D = a[s] * (s < S - 1 ? df[s] + D : df[s]);
+    }
     if constexpr (MODE == 0) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        fA[i] = A[i];
-        fB[i] = ol[0][i] * xf[0][i];
-      }
-#pragma unroll
-      for (int s = 1; s < S; ++s)
-#pragma unroll
-        for (int i = 0; i < V; ++i) fB[i] = __builtin_fmaf(a[s][i], fB[i], ol[s][i] * xf[s][i]);
-#pragma unroll
-      for (int i = 0; i < V; ++i) fin[i] = state.v[i];
+      for (int s = 0; s < S; ++s) B = s ? __builtin_fmaf(a[s], B, ol[s] * xf[s]) : ol[0] * xf[0];
     }
-    if (ch > c0) load(ch - 1);
-    float tA[V], tD[V], in[V];
-    join_lanes<false, V>(A, D, p, k, tA, tD);
-    if constexpr (NW > 1) put_waves<V>(lds[ch & 1][0], tA, tD, p);
-    if constexpr (MODE == 0) {
-      float ftA[V], ftB[V], hin[V];
-      join_lanes<true, V>(fA, fB, p, k, ftA, ftB);
-      if constexpr (NW > 1) {
-        put_waves<V>(lds[ch & 1][1], ftA, ftB, p);
-        __syncthreads();
+    float in;
+    if (p.waves > 1) {
+      down.at(ch & 1, p.wave) = make_float2(A, D);
+      if constexpr (MODE == 0) up.at(ch & 1, p.wave) = make_float2(A, B);
+      block_sync();
+      if constexpr (MODE == 0) {
+        for (int w = 0; w < p.wave; ++w) {
+          const float2 r = up.at(ch & 1, w);
+          h = __builtin_fmaf(r.x, h, r.y);
+        }
+      } else {
+        whole *= down.product(ch & 1);
       }
-      join_waves<false, V, NW>(lds[ch & 1][0], tA, tD, p, carry, in);
-      join_waves<true, V, NW>(lds[ch & 1][1], ftA, ftB, p, fin, hin);
-      float hb[S][V];
+      down.template join<false>(ch & 1, p.wave, carry, in);
+    } else {
+      in = carry;
+      carry = __builtin_fmaf(A, carry, D);
+      if constexpr (MODE == 1) whole *= A;
+    }
+    if constexpr (MODE == 0) {
+      float hb[S];
 #pragma unroll
-      for (int i = 0; i < V; ++i) hb[0][i] = __builtin_fmaf(fA[i], hin[i], fB[i]);
-#pragma unroll
-      for (int s = 1; s < S; ++s)
-#pragma unroll
-        for (int i = 0; i < V; ++i) hb[s][i] = __builtin_fmaf(a[s - 1][i], hb[s - 1][i], ol[s - 1][i] * xf[s - 1][i]);
-      float c[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) c[i] = __builtin_fmaf(A[i], in[i], D[i]);
-      Vec<T, V> dx[S];
-      Vec<G, V> dg[S];
+      for (int s = 0; s < S; ++s) {
+        hb[s] = h;
+        h = __builtin_fmaf(a[s], h, ol[s] * xf[s]);
+      }
+      T dx[S];
+      G dg[S];
 #pragma unroll
       for (int s = S - 1; s >= 0; --s) {
-        const bool lives = full || (live >> s & 1);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float gt = df[s][i] + c[i];
-          c[i] = a[s][i] * gt;
-          float vx, vg;
-          if constexpr (FORM == SB_SCAN_SIGMOID) {
-            vx = ol[s][i] * gt;
-            vg = gt * (hb[s][i] - xf[s][i]) * (a[s][i] * ol[s][i]);
-          } else {
-            vx = gt;
-            vg = gt * hb[s][i];
-          }
-          dx[s].v[i] = lives ? (T)vx : (T)0.f;
-          dg[s].v[i] = lives ? (G)vg : (G)0.f;
+        const float gt = df[s] + in;
+        in = a[s] * gt;
+        if constexpr (FORM == SB_SCAN_SIGMOID) {
+          const float vx = ol[s] * gt;
+          dx[s] = (T)vx;
+          dg[s] = (G)(vx * a[s] * (hb[s] - xf[s]));
+        } else {
+          dx[s] = (T)gt;
+          dg[s] = (G)(gt * hb[s]);
         }
       }
-      store_steps<T, V>(k.dx, dx, p, k, t0, full);
-      store_steps<G, V>(k.dgate, dg, p, k, t0, full);
-    } else {
-      if constexpr (NW > 1) {
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NW; ++w)
-#pragma unroll
-          for (int i = 0; i < V; ++i) whole[i] *= lds[ch & 1][0][w][p.lc * V + i][0];
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) whole[i] *= tA[i];
+      if (!full) {
+        kill_dead<T>(dx, live);
+        kill_dead<G>(dg, live);
       }
-      join_waves<false, V, NW>(lds[ch & 1][0], tA, tD, p, carry, in);
+      store_steps<T>(k.dx, dx, p, k, t, full);
+      store_steps<G>(k.dgate, dg, p, k, t, full);
     }
+  };
+  load(c1 - 1, start(c1 - 1), p.full(start(c1 - 1)), k.dh != nullptr);
+  for (int64_t ch = c1 - 1; ch >= c0; --ch) {
+    wait_memory();
+    if (k.dh)
+      for (; ch > c0 && p.full(start(ch)) && p.full(start(ch - 1)); --ch) chunk(ch, std::true_type());
+    chunk(ch, std::false_type());
   }
-  if (p.tseg == 0 && p.on) {
-    Vec<float, V> o, w;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      o.v[i] = carry[i];
-      w.v[i] = whole[i];
-    }
+  if (p.wave == 0 && p.on) {
     if constexpr (MODE == 0) {
-      if (split == 0 && k.dh0) vstore<float, V>(k.dh0 + oc, o);
+      if (split == 0 && k.dh0) k.dh0[p.q] = carry;
     } else {
-      vstore<float, V>(k.agg + (2 * split) * plane + oc, w);
-      vstore<float, V>(k.agg + (2 * split + 1) * plane + oc, o);
+      k.agg[(2 * split) * plane + p.q] = whole;
+      k.agg[(2 * split + 1) * plane + p.q] = carry;
     }
   }
 }
@@ -507,7 +422,8 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(const T* x, const 
   Vec<float, V> h = vload_n<float, V>(state + row * inner + c, n);
   Vec<T, V> o;
   float a[V], b[V];
-  coefficients<G, FORM, V>(gv, a, b, true);
+#pragma unroll
+  for (int i = 0; i < V; ++i) coefficients<FORM>((float)gv.v[i], a[i], b[i]);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     h.v[i] = __builtin_fmaf(a[i], h.v[i], b[i] * (float)xv.v[i]);
@@ -535,15 +451,10 @@ bool bad_sizes(int64_t outer, int64_t steps, int64_t inner) {
   return outer < 0 || steps < 0 || inner < 0 || inner > (1LL << 40) || outer > (1LL << 40) || steps > (1LL << 40);
 }
 
-void lay_args(Kargs& k, const Lay& l, int splits, int64_t keep) {
-  k.tiles = l.tiles;
-  k.cols = l.cols;
-  k.lc = l.lc;
-  k.lseg = l.lseg;
+void lay_args(Kargs& k, const Lay& l) {
   k.chunk_steps = l.steps;
-  k.chunks = (k.steps + l.steps - 1) / l.steps;
-  k.splits = splits;
-  k.keep = keep;
+  k.chunks = l.chunks;
+  k.splits = l.splits;
 }
 
 }  // namespace
@@ -553,11 +464,9 @@ extern "C" int sb_gated_scan_plan(int64_t outer, int64_t steps, int64_t inner, i
   if (bad_sizes(outer, steps, inner) || xtype < SB_F32 || xtype > SB_F16 || !chunks || !fwd_scratch || !bwd_scratch) return -1001;
   *chunks = *fwd_scratch = *bwd_scratch = 0;
   if (outer == 0 || steps == 0 || inner == 0) return 0;
-  const Lay f = fwd_lay(outer, steps, inner, xtype), b = bwd_lay(outer, steps, inner, xtype);
-  *chunks = (steps + b.steps - 1) / b.steps;
-  const int sf = splits_of(f, steps), sb = splits_of(b, steps);
-  *fwd_scratch = sf > 1 ? 2 * sf * outer * inner : 0;
-  *bwd_scratch = sb > 1 ? 2 * sb * outer * inner : 0;
+  const Lay l = lay_of(outer, steps, inner);
+  *chunks = l.chunks;
+  *fwd_scratch = *bwd_scratch = l.splits > 1 ? 2 * l.splits * outer * inner : 0;
   return 0;
 }
 
@@ -570,26 +479,20 @@ extern "C" int sb_gated_scan_fwd(const sb_gated_scan_args* ap, void* stream) {
   return with_types(a.xtype, a.gtype, a.form, [&](auto* xt, auto* gt, auto form) -> int {
     using T = std::remove_pointer_t<decltype(xt)>;
     using G = std::remove_pointer_t<decltype(gt)>;
-    const Lay l = fwd_lay(a.outer, a.steps, a.inner, a.xtype);
-    const int splits = splits_of(l, a.steps);
-    if (l.groups() > 0x7fffffffLL) return -1006;
-    if (splits > 1 && !a.scratch) return -1007;
+    const Lay l = lay_of(a.outer, a.steps, a.inner);
+    if (l.tiles > 0x7fffffffLL) return -1006;
+    if (l.splits > 1 && !a.scratch) return -1007;
     Kargs k = {};
     k.outer = a.outer; k.steps = a.steps; k.inner = a.inner; k.reverse = a.reverse != 0;
     k.x = a.x; k.so_x = a.so_x; k.st_x = a.st_x;
     k.gate = a.gate; k.so_g = a.so_g; k.st_g = a.st_g;
     k.h0 = a.h0; k.len = a.len; k.h = a.h; k.h_last = a.h_last; k.states = a.states; k.agg = a.scratch;
-    lay_args(k, l, splits, bwd_lay(a.outer, a.steps, a.inner, a.xtype).steps);
-    const auto go = [&](auto v, auto nw) {
-      constexpr int V = decltype(v)::value, NW = decltype(nw)::value;
-      if (splits > 1)
-        hipLaunchKernelGGL((gated_scan_fwd_kernel<T, G, form.value, V, NW, 1>), dim3((unsigned)l.groups(), splits - 1), dim3(64 * NW), 0, (hipStream_t)stream, k);
-      hipLaunchKernelGGL((gated_scan_fwd_kernel<T, G, form.value, V, NW, 0>), dim3((unsigned)l.groups(), splits), dim3(64 * NW), 0, (hipStream_t)stream, k);
-    };
-    const auto waves = [&](auto v) {
-      if (l.nw == 4) go(v, std::integral_constant<int, 4>()); else go(v, std::integral_constant<int, 1>());
-    };
-    if (fwd_vec(a.inner, a.xtype) == 1) waves(std::integral_constant<int, 1>()); else waves(std::integral_constant<int, vec_of<T>()>());
+    lay_args(k, l);
+    const dim3 block(64 * l.nw);
+    const unsigned lds = l.nw > 1 ? 16 * 64 * l.nw : 0;
+    if (l.splits > 1)
+      hipLaunchKernelGGL((gated_scan_fwd_kernel<T, G, form.value, 1>), dim3((unsigned)l.tiles, l.splits - 1), block, lds, (hipStream_t)stream, k);
+    hipLaunchKernelGGL((gated_scan_fwd_kernel<T, G, form.value, 0>), dim3((unsigned)l.tiles, l.splits), block, lds, (hipStream_t)stream, k);
     SB_CHECK_LAUNCH();
     return 0;
   });
@@ -604,10 +507,9 @@ extern "C" int sb_gated_scan_bwd(const sb_gated_scan_bwd_args* ap, void* stream)
   return with_types(a.xtype, a.gtype, a.form, [&](auto* xt, auto* gt, auto form) -> int {
     using T = std::remove_pointer_t<decltype(xt)>;
     using G = std::remove_pointer_t<decltype(gt)>;
-    const Lay l = bwd_lay(a.outer, a.steps, a.inner, a.xtype);
-    const int splits = splits_of(l, a.steps);
-    if (l.groups() > 0x7fffffffLL) return -1006;
-    if (splits > 1 && !a.scratch) return -1007;
+    const Lay l = lay_of(a.outer, a.steps, a.inner);
+    if (l.tiles > 0x7fffffffLL) return -1006;
+    if (l.splits > 1 && !a.scratch) return -1007;
     Kargs k = {};
     k.outer = a.outer; k.steps = a.steps; k.inner = a.inner; k.reverse = a.reverse != 0;
     k.x = a.x; k.so_x = a.so_x; k.st_x = a.st_x;
@@ -615,17 +517,12 @@ extern "C" int sb_gated_scan_bwd(const sb_gated_scan_bwd_args* ap, void* stream)
     k.dh = a.dh; k.so_d = a.so_d; k.st_d = a.st_d;
     k.dlast = a.dlast; k.len = a.len; k.states = const_cast<float*>(a.states); k.agg = a.scratch;
     k.dx = a.dx; k.dgate = a.dgate; k.dh0 = a.dh0;
-    lay_args(k, l, splits, l.steps);
-    const auto go = [&](auto v, auto nw) {
-      constexpr int V = decltype(v)::value, NW = decltype(nw)::value;
-      if (splits > 1)
-        hipLaunchKernelGGL((gated_scan_bwd_kernel<T, G, form.value, V, NW, 1>), dim3((unsigned)l.groups(), splits - 1), dim3(64 * NW), 0, (hipStream_t)stream, k);
-      hipLaunchKernelGGL((gated_scan_bwd_kernel<T, G, form.value, V, NW, 0>), dim3((unsigned)l.groups(), splits), dim3(64 * NW), 0, (hipStream_t)stream, k);
-    };
-    const auto waves = [&](auto v) {
-      if (l.nw == 4) go(v, std::integral_constant<int, 4>()); else go(v, std::integral_constant<int, 1>());
-    };
-    if (bwd_vec(a.inner) == 1) waves(std::integral_constant<int, 1>()); else waves(std::integral_constant<int, 4>());
+    lay_args(k, l);
+    const dim3 block(64 * l.nw);
+    const unsigned lds = l.nw > 1 ? 32 * 64 * l.nw : 0;
+    if (l.splits > 1)
+      hipLaunchKernelGGL((gated_scan_bwd_kernel<T, G, form.value, 1>), dim3((unsigned)l.tiles, l.splits - 1), block, lds, (hipStream_t)stream, k);
+    hipLaunchKernelGGL((gated_scan_bwd_kernel<T, G, form.value, 0>), dim3((unsigned)l.tiles, l.splits), block, lds, (hipStream_t)stream, k);
     SB_CHECK_LAUNCH();
     return 0;
   });
