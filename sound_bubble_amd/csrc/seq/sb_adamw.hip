@@ -2,12 +2,15 @@
 //
 // A launch's tensors come as a table in the kernel's arguments; a workgroup takes chunks of kChunk elements, a wave blocks of 256
 // (4 elements a lane), the unit that shares a scale where the states are in 8 bits.  Every operation is rounded by itself (the file is
-// compiled without contraction), so that the value a code is made from is the formula's own.
+// compiled without contraction), so that the value a code is made from is the formula's own; the update itself, which no code is made
+// from, takes the hardware's square root and reciprocal (1 ulp each; v below 2^-126 counts as 0 in it).
 #include "sb_seq_common.h"
 
 namespace {
 
-constexpr int kBlock = SB_ADAMW_BLOCK, kChunk = 4096, kPerWave = kChunk / kBlock / 4;      // blocks of a wave in a chunk
+constexpr int kBlock = SB_ADAMW_BLOCK, kChunk = 8192, kPerWave = kChunk / kBlock / 4;      // blocks of a wave in a chunk
+constexpr int kTogether = 4;      // blocks whose loads are under way together
+constexpr int kNormThreads = 512;
 static_assert(kBlock == 64 * 4, "a wave holds a block");
 
 SB_DEVINL double wave_sum_f64(double v) {
@@ -15,18 +18,25 @@ SB_DEVINL double wave_sum_f64(double v) {
   for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, 64);
   return v;
 }
-// sum over the workgroup's 4 waves, in every thread
-SB_DEVINL double block_sum_f64(double v, double* lds) {
+// sum over the workgroup's N waves, in every thread
+template <int N> SB_DEVINL double block_sum_f64(double v, double* lds) {
   v = wave_sum_f64(v);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
-}
-// the largest bit pattern of |x| in the wave: NaN and infinity come out on top
-SB_DEVINL unsigned wave_max_bits(unsigned v) {
+  double s = 0.0;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) v = max(v, (unsigned)__shfl_xor((int)v, d, 64));
-  return v;
+  for (int w = 0; w < N; ++w) s += lds[w];
+  return s;
+}
+// the largest bit pattern of |x| in the wave, uniform: NaN and infinity come out on top
+template <int CTRL> SB_DEVINL unsigned dpp_max(unsigned v) { return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false)); }
+SB_DEVINL unsigned wave_max_bits(unsigned v) {
+  v = dpp_max<0xB1>(v);      // quad_perm [1,0,3,2]
+  v = dpp_max<0x4E>(v);      // quad_perm [2,3,0,1]
+  v = dpp_max<0x141>(v);     // row_half_mirror
+  v = dpp_max<0x140>(v);     // row_mirror
+  const unsigned a = max((unsigned)__builtin_amdgcn_readlane((int)v, 0), (unsigned)__builtin_amdgcn_readlane((int)v, 16));
+  return max(a, max((unsigned)__builtin_amdgcn_readlane((int)v, 32), (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
 }
 
 // the tensor that chunk `c` of the launch belongs to
@@ -39,25 +49,35 @@ SB_DEVINL int tensor_of(const sb_adamw_args& a, int c) {
   return lo;
 }
 
-template <class G> __global__ __launch_bounds__(256) void adamw_norm_kernel(sb_adamw_args a, double* part, int chunks) {
-  __shared__ double lds[4];
+template <class G> __global__ __launch_bounds__(kNormThreads) void adamw_norm_kernel(sb_adamw_args a, double* part, int chunks) {
+  __shared__ double lds[kNormThreads / 64];
+  constexpr int V = vec_of<G>(), N = kChunk / kNormThreads / V;
   double s = 0.0;
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     const sb_adamw_tensor& t = a.t[tensor_of(a, c)];
     const int64_t i0 = (int64_t)(c - t.first_chunk) * kChunk;
-    const G* g = (const G*)t.g;
+    const G* g = (const G*)t.g + i0;
+    const int n = (int)min(t.n - i0, (int64_t)kChunk);
+    Vec<G, V> v[N];
+    if (n == kChunk) {
 #pragma unroll
-    for (int j = 0; j < kChunk / 1024; ++j) {
-      const int64_t i = i0 + j * 1024 + threadIdx.x * 4;
-      const Vec<G, 4> v = vload_n<G, 4>(g + i, (int)min(max(t.n - i, (int64_t)0), (int64_t)4));
+      for (int j = 0; j < N; ++j) v[j] = vload<G, V>(g + (j * kNormThreads + threadIdx.x) * V);
+    } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const double d = (double)(float)v.v[k];
-        s += d * d;
+      for (int j = 0; j < N; ++j) {
+        const int i = (j * kNormThreads + threadIdx.x) * V;
+        v[j] = vload_n<G, V>(g + i, max(n - i, 0));
       }
     }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const double d = (double)(float)v[j].v[k];
+        s += d * d;
+      }
   }
-  s = block_sum_f64(s, lds);
+  s = block_sum_f64<kNormThreads / 64>(s, lds);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
@@ -86,8 +106,9 @@ template <int M, int BIAS, int TOP> struct Float8 {
     constexpr int CUT = 23 - M;
     const unsigned add = (u16 << (CUT - 16)) + (1u << (CUT - 17));
     constexpr float lowest = 1.f / (float)(1 << (BIAS - 1));
-    if (y >= lowest) return (((unsigned)__float_as_int(y) + add) >> CUT) - ((127 - BIAS) << M);
-    return ((unsigned)(y * __int_as_float((127 + BIAS - 1 + M + CUT) << 23)) + add) >> CUT;
+    const unsigned normal = (((unsigned)__float_as_int(y) + add) >> CUT) - ((127 - BIAS) << M);
+    const unsigned small = ((unsigned)(y * __int_as_float((127 + BIAS - 1 + M + CUT) << 23)) + add) >> CUT;
+    return y >= lowest ? normal : small;
   }
 };
 using E4M3 = Float8<3, 7, 8>;
@@ -121,12 +142,108 @@ SB_DEVINL Rates rates_of(const sb_adamw_args& a, double* lds) {
   if (a.clip > 0.f) {
     double s = 0.0;
     for (int i = threadIdx.x; i < a.norm_slots; i += 256) s += a.norm_part[i];
-    const float norm = sqrtf((float)block_sum_f64(s, lds)) * a.gscale;
+    const float norm = sqrtf((float)block_sum_f64<4>(s, lds)) * a.gscale;
     const float coef = a.clip / (norm + 1e-6f);
     r.gscale *= coef > 1.f ? 1.f : coef;      // (a NaN norm stays one)
   }
   return r;
 }
+
+// Read once and written once: streams past the caches.  96 M bf16 parameters with fp32 states, us: plain 640, stores so 626, loads too 546
+template <class E> SB_DEVINL Vec<E, 4> stream_load(const E* p) {
+  typedef E x4 __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+  const x4 v = __builtin_nontemporal_load((const x4*)p);
+  return {v[0], v[1], v[2], v[3]};
+}
+template <class E> SB_DEVINL void stream_store(E* p, const Vec<E, 4>& o) {
+  typedef E x4 __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+  const x4 v = {o.v[0], o.v[1], o.v[2], o.v[3]};
+  __builtin_nontemporal_store(v, (x4*)p);
+}
+
+// what a lane holds of a block: 4 elements
+template <class P, class G, int BITS> struct Part {
+  static constexpr bool kMaster = !std::is_same_v<P, float>;
+  Vec<G, 4> g;
+  Vec<float, 4> p, m, v;
+  int mc, vc, ms, vs;
+
+  // n: elements that exist, 4 where FULL
+  template <bool FULL> SB_DEVINL void load(const sb_adamw_args& a, const P* pp, const G* gp, int64_t i, int64_t s, int n) {
+    g = FULL ? stream_load(gp + i) : vload_n<G, 4>(gp + i, n);
+    const float* from = kMaster ? a.master + s : (const float*)pp + i;
+    p = FULL ? stream_load(from) : vload_n<float, 4>(from, n);
+    if constexpr (BITS == 32) {
+      m = FULL ? stream_load((const float*)a.m + s) : vload_n<float, 4>((const float*)a.m + s, n);
+      v = FULL ? stream_load((const float*)a.v + s) : vload_n<float, 4>((const float*)a.v + s, n);
+    } else {      // (the buffers have whole blocks)
+      mc = __builtin_nontemporal_load((const int*)((const uint8_t*)a.m + s));
+      vc = __builtin_nontemporal_load((const int*)((const uint8_t*)a.v + s));
+      ms = ((const uint8_t*)a.m_scale)[s / kBlock];
+      vs = ((const uint8_t*)a.v_scale)[s / kBlock];
+    }
+  }
+  SB_DEVINL void step(const Rates& r, int n) {
+    if constexpr (BITS == 8) {
+      const float mf = E4M3::scale(ms), vf = E5M2::scale(vs);
+      m.v[0] = __builtin_amdgcn_cvt_f32_fp8(mc, 0) * mf;
+      m.v[1] = __builtin_amdgcn_cvt_f32_fp8(mc, 1) * mf;
+      m.v[2] = __builtin_amdgcn_cvt_f32_fp8(mc, 2) * mf;
+      m.v[3] = __builtin_amdgcn_cvt_f32_fp8(mc, 3) * mf;
+      v.v[0] = __builtin_amdgcn_cvt_f32_bf8(vc, 0) * vf;
+      v.v[1] = __builtin_amdgcn_cvt_f32_bf8(vc, 1) * vf;
+      v.v[2] = __builtin_amdgcn_cvt_f32_bf8(vc, 2) * vf;
+      v.v[3] = __builtin_amdgcn_cvt_f32_bf8(vc, 3) * vf;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = (float)g.v[k] * r.gscale;
+      m.v[k] = m.v[k] * r.b1 + f * r.c1;
+      v.v[k] = v.v[k] * r.b2 + (f * f) * r.c2;
+      p.v[k] = p.v[k] * r.decay - r.rate * (m.v[k] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v.v[k]) * r.root2 + r.eps));
+      if (k >= n) m.v[k] = v.v[k] = 0.f;
+    }
+  }
+  template <bool FULL> SB_DEVINL void store(const sb_adamw_args& a, const Rates& r, P* pp, int64_t i, int64_t s, int n) {
+    if constexpr (kMaster) {
+      Vec<P, 4> o;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o.v[k] = (P)p.v[k];
+      if constexpr (FULL) stream_store(pp + i, o); else vstore_n<P, 4>(pp + i, o, n);
+    }
+    float* to = kMaster ? a.master + s : (float*)pp + i;
+    if constexpr (FULL) stream_store(to, p); else vstore_n<float, 4>(to, p, n);
+    if constexpr (BITS == 32) {
+      if constexpr (FULL) stream_store((float*)a.m + s, m); else vstore_n<float, 4>((float*)a.m + s, m, n);
+      if constexpr (FULL) stream_store((float*)a.v + s, v); else vstore_n<float, 4>((float*)a.v + s, v, n);
+    } else {
+      unsigned mb = 0, vb = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        mb = max(mb, (unsigned)__float_as_int(m.v[k]) & 0x7FFFFFFFu);
+        vb = max(vb, (unsigned)__float_as_int(v.v[k]) & 0x7FFFFFFFu);
+      }
+      const int mscale = E4M3::scale_byte(wave_max_bits(mb)), vscale = E5M2::scale_byte(wave_max_bits(vb));
+      unsigned mq = 0, vq = 0;
+      const float mi = E4M3::inverse(mscale), vi = E5M2::inverse(vscale);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned u = dither(s + k, r.key);
+        unsigned q = E4M3::code(__builtin_fabsf(m.v[k]) * mi, u & 0xFFFFu) | ((unsigned)__float_as_int(m.v[k]) >> 31 << 7);
+        mq |= (mscale == 255 ? 0u : q) << (8 * k);
+        q = E5M2::code(v.v[k] * vi, u >> 16);
+        if (q == 0 && v.v[k] > 0.f) q = 1;
+        vq |= (vscale == 255 ? 0u : q) << (8 * k);
+      }
+      *(unsigned*)((uint8_t*)a.m + s) = mq;
+      *(unsigned*)((uint8_t*)a.v + s) = vq;
+      if ((threadIdx.x & 63) == 0) {
+        ((uint8_t*)a.m_scale)[s / kBlock] = (uint8_t)mscale;
+        ((uint8_t*)a.v_scale)[s / kBlock] = (uint8_t)vscale;
+      }
+    }
+  }
+};
 
 template <class P, class G, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(sb_adamw_args a, int chunks) {
@@ -136,86 +253,29 @@ __global__ __launch_bounds__(256) void adamw_kernel(sb_adamw_args a, int chunks)
     return;
   }
   const Rates r = rates_of(a, lds);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr bool kMaster = !std::is_same_v<P, float>;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     const sb_adamw_tensor& t = a.t[tensor_of(a, c)];
     const int64_t i0 = (int64_t)(c - t.first_chunk) * kChunk + wave * (kPerWave * kBlock);
     const int64_t s0 = (int64_t)t.first_block * kBlock + i0;
     P* pp = (P*)t.p;
     const G* gp = (const G*)t.g;
-#pragma unroll
-    for (int j = 0; j < kPerWave; ++j) {
+    for (int j = 0; j < kPerWave && i0 + j * kBlock < t.n; j += kTogether) {
       const int64_t i = i0 + j * kBlock + lane * 4, s = s0 + j * kBlock + lane * 4;
-      if (i0 + j * kBlock >= t.n) break;      // (the whole wave)
-      const int n = (int)min(max(t.n - i, (int64_t)0), (int64_t)4);
-      const Vec<G, 4> gv = vload_n<G, 4>(gp + i, n);
-      Vec<float, 4> p, m, v;
-      if constexpr (kMaster) {
-        p = vload_n<float, 4>(a.master + s, n);
-      } else {
-        p = vload_n<float, 4>(pp + i, n);
-      }
-      if constexpr (BITS == 32) {
-        m = vload_n<float, 4>((const float*)a.m + s, n);
-        v = vload_n<float, 4>((const float*)a.v + s, n);
-      } else {
-        const int mc = *(const int*)((const uint8_t*)a.m + s), vc = *(const int*)((const uint8_t*)a.v + s);
-        const float ms = E4M3::scale(((const uint8_t*)a.m_scale)[s / kBlock]), vs = E5M2::scale(((const uint8_t*)a.v_scale)[s / kBlock]);
-        m.v[0] = __builtin_amdgcn_cvt_f32_fp8(mc, 0) * ms;
-        m.v[1] = __builtin_amdgcn_cvt_f32_fp8(mc, 1) * ms;
-        m.v[2] = __builtin_amdgcn_cvt_f32_fp8(mc, 2) * ms;
-        m.v[3] = __builtin_amdgcn_cvt_f32_fp8(mc, 3) * ms;
-        v.v[0] = __builtin_amdgcn_cvt_f32_bf8(vc, 0) * vs;
-        v.v[1] = __builtin_amdgcn_cvt_f32_bf8(vc, 1) * vs;
-        v.v[2] = __builtin_amdgcn_cvt_f32_bf8(vc, 2) * vs;
-        v.v[3] = __builtin_amdgcn_cvt_f32_bf8(vc, 3) * vs;
-      }
+      Part<P, G, BITS> part[kTogether];
+      if (i0 + (j + kTogether) * kBlock <= t.n) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float g = (float)gv.v[k] * r.gscale;
-        m.v[k] = m.v[k] * r.b1 + g * r.c1;
-        v.v[k] = v.v[k] * r.b2 + (g * g) * r.c2;
-        const float u = m.v[k] / (sqrtf(v.v[k]) * r.root2 + r.eps);
-        p.v[k] = p.v[k] * r.decay - r.rate * u;
-        if (k >= n) m.v[k] = v.v[k] = 0.f;
-      }
-      if constexpr (kMaster) {
-        vstore_n<float, 4>(a.master + s, p, n);
-        Vec<P, 4> o;
+        for (int b = 0; b < kTogether; ++b) part[b].template load<true>(a, pp, gp, i + b * kBlock, s + b * kBlock, 4);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o.v[k] = (P)p.v[k];
-        vstore_n<P, 4>(pp + i, o, n);
+        for (int b = 0; b < kTogether; ++b) part[b].step(r, 4);
+#pragma unroll
+        for (int b = 0; b < kTogether; ++b) part[b].template store<true>(a, r, pp, i + b * kBlock, s + b * kBlock, 4);
       } else {
-        vstore_n<float, 4>(pp + i, p, n);
-      }
-      if constexpr (BITS == 32) {
-        vstore_n<float, 4>((float*)a.m + s, m, n);
-        vstore_n<float, 4>((float*)a.v + s, v, n);
-      } else {
-        unsigned mb = 0, vb = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          mb = max(mb, (unsigned)__float_as_int(m.v[k]) & 0x7FFFFFFFu);
-          vb = max(vb, (unsigned)__float_as_int(v.v[k]) & 0x7FFFFFFFu);
-        }
-        const int ms = E4M3::scale_byte(wave_max_bits(mb)), vs = E5M2::scale_byte(wave_max_bits(vb));
-        unsigned mc = 0, vc = 0;
-        const float mi = E4M3::inverse(ms), vi = E5M2::inverse(vs);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const unsigned u = dither(s + k, r.key);
-          unsigned q = E4M3::code(__builtin_fabsf(m.v[k]) * mi, u & 0xFFFFu) | ((unsigned)__float_as_int(m.v[k]) >> 31 << 7);
-          mc |= (ms == 255 ? 0u : q) << (8 * k);
-          q = E5M2::code(v.v[k] * vi, u >> 16);
-          if (q == 0 && v.v[k] > 0.f) q = 1;
-          vc |= (vs == 255 ? 0u : q) << (8 * k);
-        }
-        *(unsigned*)((uint8_t*)a.m + s) = mc;
-        *(unsigned*)((uint8_t*)a.v + s) = vc;
-        if (lane == 0) {
-          ((uint8_t*)a.m_scale)[s / kBlock] = (uint8_t)ms;
-          ((uint8_t*)a.v_scale)[s / kBlock] = (uint8_t)vs;
+        for (int b = 0; b < kTogether && i0 + (j + b) * kBlock < t.n; ++b) {      // (the whole wave)
+          const int n = (int)min(max(t.n - i - b * kBlock, (int64_t)0), (int64_t)4);
+          part[0].template load<false>(a, pp, gp, i + b * kBlock, s + b * kBlock, n);
+          part[0].step(r, n);
+          part[0].template store<false>(a, r, pp, i + b * kBlock, s + b * kBlock, n);
         }
       }
     }
@@ -235,7 +295,7 @@ int64_t chunks_of(const sb_adamw_args& a, bool step) {
   return chunks;
 }
 
-constexpr int kGrid = 2048;
+constexpr int kGrid = 4096;
 
 }  // namespace
 
@@ -247,7 +307,7 @@ extern "C" int sb_adamw_norm(const sb_adamw_args* a, double* norm_part, int slot
   if (chunks < 0) return (int)chunks;
   return sb_with_type(a->gtype, [&](auto* t) -> int {
     using G = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL((adamw_norm_kernel<G>), dim3(slots), dim3(256), 0, (hipStream_t)stream, *a, norm_part + slot0, (int)chunks);
+    hipLaunchKernelGGL((adamw_norm_kernel<G>), dim3(slots), dim3(kNormThreads), 0, (hipStream_t)stream, *a, norm_part + slot0, (int)chunks);
     SB_CHECK_LAUNCH();
     return 0;
   });
