@@ -5,9 +5,10 @@ float32, bfloat16 and float16 on a HIP device; anything else raises, there is no
 stream of the tensors' own device; what a call needs besides its results is allocated for the call.
 """
 import ctypes as C
+import functools
 import itertools
-import struct
 
+import numpy as np
 import torch
 
 from . import _lib as L
@@ -35,22 +36,23 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """the tensors' own device for the launches inside, and its current stream"""
+def _launch(fn, device, *args):
+    """fn(*args, stream) on the tensors' own device and its current stream (ops.on_stream's, inside one)"""
+    from . import ops
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _launch(fn, device, *args)
+    stream = ops._STREAM_OVERRIDE
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(index)
+    rc = fn(*args, stream)
+    if rc:
+        L.check(rc, fn.__name__)
 
-    def __init__(self, device):
-        self.ctx = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
 
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        from . import ops
-        return ops._stream()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-        return False
+def _like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 # ---- layer norm ----
@@ -81,10 +83,10 @@ def layer_norm_fwd(x, weight, bias, eps=1e-5, stats=True):
     shape (None without `stats`).  weight / bias (None: 1 / 0) in x's type or float32."""
     _need(x, "layer_norm: x", _TYPES)
     n = _norm_params(x, weight, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _like(x)
     mean = rstd = None
     if stats:
-        mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device).unbind(0)
+        mean, rstd = x.new_empty((2,) + x.shape[:-1], dtype=torch.float32).unbind(0)
     rows = x.numel() // n
     if rows == 0:
         return y, mean, rstd
@@ -93,8 +95,7 @@ def layer_norm_fwd(x, weight, bias, eps=1e-5, stats=True):
     wt = w if w is not None else b
     a = L.LayerNormArgs(rows, n, ldx, _TYPES[x.dtype], _TYPES[wt.dtype] if wt is not None else 0, eps, xr.data_ptr(), _ptr(w), _ptr(b),
                         y.data_ptr(), _ptr(mean), _ptr(rstd))
-    with _On(x.device) as stream:
-        L.check(L.load().sb_layer_norm_fwd(a, stream), "sb_layer_norm_fwd")
+    _launch(L.load().sb_layer_norm_fwd, x.device, a)
     return y, mean, rstd
 
 
@@ -108,22 +109,21 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, want_dw=True, want_db=True, wdtype
         if not _need(t, f"layer_norm_bwd: {name}", (torch.float32,), x.device, x.shape[:-1]).is_contiguous():
             _fail(f"layer_norm_bwd: {name} must be contiguous")
     wdtype = weight.dtype if weight is not None else (wdtype or x.dtype)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = torch.empty(n, dtype=wdtype, device=x.device) if want_dw else None
-    db = torch.empty(n, dtype=wdtype, device=x.device) if want_db else None
+    dx = _like(x)
+    dw = x.new_empty(n, dtype=wdtype) if want_dw else None
+    db = x.new_empty(n, dtype=wdtype) if want_db else None
     rows = x.numel() // n
     xt = _TYPES[x.dtype]
     lib = L.load()
     scratch = None
     if (want_dw or want_db) and rows:
-        scratch = torch.empty(lib.sb_layer_norm_bwd_scratch(rows, n, xt), dtype=torch.float32, device=x.device)
+        scratch = x.new_empty(lib.sb_layer_norm_bwd_scratch(rows, n, xt), dtype=torch.float32)
     (xr, ldx), (dyr, lddy) = _rows(x, n), _rows(dy, n)
     w = weight.contiguous() if weight is not None else None
     a = L.LayerNormBwdArgs(rows, n, ldx, lddy, xt, _TYPES[wdtype], xr.data_ptr(), dyr.data_ptr(), _ptr(w), mean.data_ptr(), rstd.data_ptr(),
                            dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(scratch))
     if rows or want_dw or want_db:
-        with _On(x.device) as stream:
-            L.check(lib.sb_layer_norm_bwd(a, stream), "sb_layer_norm_bwd")
+        _launch(lib.sb_layer_norm_bwd, x.device, a)
     return dx, dw, db
 
 
@@ -155,10 +155,12 @@ def _scan_sizes(x, gate, dim, form, h0, lengths):
     return dim, rest, outer, x.shape[dim], x.shape[dim + 1:].numel()
 
 
+@functools.lru_cache(maxsize=256)
 def _scan_plan(outer, steps, inner, xt):
+    """(a function of the sizes alone)"""
     got = [C.c_int64() for _ in range(3)]
     L.check(L.load().sb_gated_scan_plan(outer, steps, inner, xt, *(C.byref(v) for v in got)), "sb_gated_scan_plan")
-    return [v.value for v in got]
+    return tuple(v.value for v in got)
 
 
 def gated_scan_fwd(x, gate, h0=None, *, dim=1, form="sigmoid", reverse=False, lengths=None, save=True):
@@ -167,23 +169,22 @@ def gated_scan_fwd(x, gate, h0=None, *, dim=1, form="sigmoid", reverse=False, le
     lengths (int64 / int32, x.shape[:dim]): steps behind a sequence's length leave its state alone and give 0.
     states (None without `save`): what gated_scan_bwd needs, fp32."""
     dim, rest, outer, steps, inner = _scan_sizes(x, gate, dim, form, h0, lengths)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = _like(x)
     if x.numel() == 0:
         last = torch.zeros(rest, dtype=torch.float32, device=x.device) if h0 is None else h0.clone()
         return h, last, torch.empty(0, dtype=torch.float32, device=x.device) if save else None
-    last = torch.empty(rest, dtype=torch.float32, device=x.device)
+    last = x.new_empty(rest, dtype=torch.float32)
     xt = _TYPES[x.dtype]
     chunks, scratch_n, _ = _scan_plan(outer, steps, inner, xt)
-    states = torch.empty(chunks * outer * inner, dtype=torch.float32, device=x.device) if save else None
-    scratch = torch.empty(scratch_n, dtype=torch.float32, device=x.device) if scratch_n else None
+    states = x.new_empty(chunks * outer * inner, dtype=torch.float32) if save else None
+    scratch = x.new_empty(scratch_n, dtype=torch.float32) if scratch_n else None
     x3, so_x, st_x = _steps(x, outer, steps, inner)
     g3, so_g, st_g = _steps(gate, outer, steps, inner)
     h0 = h0.contiguous() if h0 is not None else None
     lengths = lengths.to(torch.int64).contiguous() if lengths is not None else None
     a = L.GatedScanArgs(outer, steps, inner, xt, _TYPES[gate.dtype], FORMS[form], int(bool(reverse)), x3.data_ptr(), so_x, st_x,
                         g3.data_ptr(), so_g, st_g, _ptr(h0), _ptr(lengths), h.data_ptr(), last.data_ptr(), _ptr(states), _ptr(scratch))
-    with _On(x.device) as stream:
-        L.check(L.load().sb_gated_scan_fwd(a, stream), "sb_gated_scan_fwd")
+    _launch(L.load().sb_gated_scan_fwd, x.device, a)
     return h, last, states
 
 
@@ -195,8 +196,8 @@ def gated_scan_bwd(dh, dlast, x, gate, states, *, dim=1, form="sigmoid", reverse
         _need(dh, "gated_scan_bwd: dh", (x.dtype,), x.device, x.shape)
     if dlast is not None:
         _need(dlast, "gated_scan_bwd: dlast", (torch.float32,), x.device, rest)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dgate = torch.empty(x.shape, dtype=gate.dtype, device=x.device)
+    dx = _like(x)
+    dgate = _like(gate)
     if x.numel() == 0:
         dh0 = None
         if want_dh0:
@@ -205,8 +206,8 @@ def gated_scan_bwd(dh, dlast, x, gate, states, *, dim=1, form="sigmoid", reverse
     xt = _TYPES[x.dtype]
     chunks, _, scratch_n = _scan_plan(outer, steps, inner, xt)
     _need(states, "gated_scan_bwd: states", (torch.float32,), x.device, (chunks * outer * inner,))
-    dh0 = torch.empty(rest, dtype=torch.float32, device=x.device) if want_dh0 else None
-    scratch = torch.empty(scratch_n, dtype=torch.float32, device=x.device) if scratch_n else None
+    dh0 = x.new_empty(rest, dtype=torch.float32) if want_dh0 else None
+    scratch = x.new_empty(scratch_n, dtype=torch.float32) if scratch_n else None
     x3, so_x, st_x = _steps(x, outer, steps, inner)
     g3, so_g, st_g = _steps(gate, outer, steps, inner)
     d3, so_d, st_d = _steps(dh, outer, steps, inner) if dh is not None else (None, 0, 0)
@@ -215,8 +216,7 @@ def gated_scan_bwd(dh, dlast, x, gate, states, *, dim=1, form="sigmoid", reverse
     a = L.GatedScanBwdArgs(outer, steps, inner, xt, _TYPES[gate.dtype], FORMS[form], int(bool(reverse)), x3.data_ptr(), so_x, st_x,
                            g3.data_ptr(), so_g, st_g, _ptr(d3), so_d, st_d, _ptr(dlast), _ptr(lengths), states.contiguous().data_ptr(),
                            dx.data_ptr(), dgate.data_ptr(), _ptr(dh0), _ptr(scratch))
-    with _On(x.device) as stream:
-        L.check(L.load().sb_gated_scan_bwd(a, stream), "sb_gated_scan_bwd")
+    _launch(L.load().sb_gated_scan_bwd, x.device, a)
     return dx, dgate, dh0
 
 
@@ -229,14 +229,13 @@ def gated_scan_step(x, gate, state, *, form="sigmoid"):
         _fail(f"gated_scan_step: form is one of {sorted(FORMS)}, got {form!r}")
     if not state.is_contiguous():
         _fail("gated_scan_step: state is updated in place and must be contiguous")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _like(x)
     if x.numel() == 0:
         return y
     n = x.shape[-1] if x.dim() else 1
     (xr, ldx), (gr, ldg) = _rows(x, n), _rows(gate, n)
-    with _On(x.device) as stream:
-        L.check(L.load().sb_gated_scan_step(xr.data_ptr(), gr.data_ptr(), state.data_ptr(), y.data_ptr(), x.numel() // n, n, ldx, ldg,
-                                            _TYPES[x.dtype], _TYPES[gate.dtype], FORMS[form], stream), "sb_gated_scan_step")
+    _launch(L.load().sb_gated_scan_step, x.device, xr.data_ptr(), gr.data_ptr(), state.data_ptr(), y.data_ptr(), x.numel() // n, n, ldx, ldg,
+            _TYPES[x.dtype], _TYPES[gate.dtype], FORMS[form])
     return y
 
 
@@ -272,6 +271,31 @@ def adamw_state(params, bits=32):
     return st
 
 
+_ROW = np.dtype([("p", "u8"), ("g", "u8"), ("n", "i8"), ("first_block", "i4"), ("first_chunk", "i4")])      # sb_adamw_tensor
+
+
+@functools.lru_cache(maxsize=32)
+def _adamw_layout(sizes, take, ptypes, gtypes):
+    """-> (blocks of the state buffers, [(ptype, gtype, places among the taken tensors (None: all of them), table rows)]): one entry a
+    launch, tensors of one pair of types, pointers left open.  A function of the sizes and types alone."""
+    chunk = L.load().sb_adamw_chunk()
+    starts = adamw_blocks(sizes)
+    take = range(len(sizes)) if take is None else take
+    groups = {}
+    for j, key in enumerate(zip(ptypes, gtypes)):
+        groups.setdefault(key, []).append(j)
+    out = []
+    for (pt, gt), js in groups.items():
+        for k in range(0, len(js), L.ADAMW_MAX):
+            ids, at = js[k:k + L.ADAMW_MAX], 0
+            rows = np.zeros(len(ids), dtype=_ROW)
+            for r, j in zip(rows, ids):
+                r["n"], r["first_block"], r["first_chunk"] = sizes[take[j]], min(starts[take[j]], (1 << 31) - 1), at
+                at += (sizes[take[j]] + chunk - 1) // chunk
+            out.append((pt, gt, None if len(ids) == len(take) else np.array(ids), rows))
+    return starts[-1], out
+
+
 def _adamw_check_state(state, blocks, device, need_master):
     n = blocks * L.ADAMW_BLOCK
     eight = isinstance(state.get("exp_avg"), torch.Tensor) and state["exp_avg"].dtype == torch.float8_e4m3fn
@@ -302,26 +326,31 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
     if not params:
         return
     dev = params[0].device
-    sizes = [p.numel() for p in params]
-    starts = adamw_blocks(sizes)
-    need_master = False
-    groups = {}
-    for i, (p, g) in enumerate(zip(params, grads)):
-        t = p.dtype
-        if t not in _TYPES or not p.is_cuda or p.device != dev or not p.is_contiguous():
-            _fail(f"adamw_step: parameter {i}: expected a contiguous float32 / bfloat16 / float16 tensor on {dev}, got {t} on {p.device}"
-                  f"{'' if p.is_contiguous() else ', not contiguous'}")
-        need_master |= t != torch.float32
-        if g is None or sizes[i] == 0:
-            continue
-        gt = g.dtype
-        if (gt != t and gt != torch.float32) or g.device != dev or g.numel() != sizes[i] or g.shape != p.shape:
-            _fail(f"adamw_step: gradient {i}: expected {t} or float32 of shape {tuple(p.shape)} on {dev}, got {gt} {tuple(g.shape)} on {g.device}")
-        if not g.is_contiguous():
-            g = grads[i] = g.contiguous()
-        groups.setdefault((t, gt), []).append(i)
-    bits = _adamw_check_state(state, starts[-1], dev, need_master)
-    if starts[-1] >= 1 << 31:
+    index, T = params[0].get_device(), torch.Tensor
+    ptypes = [p.dtype for p in params]
+    if index < 0 or {*map(T.get_device, params)} != {index} or not _TYPES.keys() >= {*ptypes} or not all(map(T.is_contiguous, params)):
+        i = next(i for i, p in enumerate(params) if not (p.is_cuda and p.device == dev and p.dtype in _TYPES and p.is_contiguous()))
+        _fail(f"adamw_step: parameter {i}: expected a contiguous float32 / bfloat16 / float16 tensor on one GPU, got {params[i].dtype} on "
+              f"{params[i].device}{'' if params[i].is_contiguous() else ', not contiguous'}")
+    sizes = tuple(map(T.numel, params))
+    if any(g is None for g in grads) or 0 in sizes:
+        take = tuple(i for i, g in enumerate(grads) if g is not None and sizes[i])
+        ps, gs, pts = [params[i] for i in take], [grads[i] for i in take], [ptypes[i] for i in take]
+    else:
+        take, ps, gs, pts = None, params, grads, ptypes
+    gtypes = [g.dtype for g in gs]
+    if {*map(T.get_device, gs)} - {index} or not all(map(T.is_same_size, ps, gs)) or \
+            (gtypes != pts and any(a is not b and a is not torch.float32 for a, b in zip(gtypes, pts))):
+        i, p, g = next((i, p, g) for i, (p, g) in enumerate(zip(ps, gs)) if not (g.is_cuda and g.device == dev and g.shape == p.shape and
+                                                                               g.dtype in (p.dtype, torch.float32)))
+        _fail(f"adamw_step: gradient {take[i] if take else i}: expected {p.dtype} or float32 of shape {tuple(p.shape)} on {dev}, got {g.dtype} "
+              f"{tuple(g.shape)} on {g.device}")
+    if not all(map(T.is_contiguous, gs)):
+        gs = [g.contiguous() for g in gs]
+    blocks, batches = _adamw_layout(sizes, take, tuple(map(_TYPES.get, pts)), tuple(map(_TYPES.get, gtypes)))
+    need_master = {*ptypes} != {torch.float32}
+    bits = _adamw_check_state(state, blocks, dev, need_master)
+    if blocks >= 1 << 31:
         _fail("adamw_step: more than 2^31 blocks of states")
     step_dev = lr_dev = None
     if isinstance(step, torch.Tensor):
@@ -338,20 +367,17 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
             _fail("adamw_step: lr is one number")
     if clip < 0:
         _fail(f"adamw_step: clip is a norm (0: none), got {clip}")
-    lib = L.load()
-    chunk = lib.sb_adamw_chunk()
-    batches = [(key, ids[j:j + L.ADAMW_MAX]) for key, ids in groups.items() for j in range(0, len(ids), L.ADAMW_MAX)]
     if not batches:
         return
+    lib = L.load()
+    pp, gp = (np.array([*map(T.data_ptr, ts)], dtype=np.uint64) for ts in (ps, gs))
     calls = []
-    for (t, gt), ids in batches:
+    for pt, gt, ids, rows in batches:
         a = L.AdamwArgs()
-        row, at = [], 0
-        for i in ids:
-            row += (params[i].data_ptr(), grads[i].data_ptr(), sizes[i], starts[i], at)
-            at += (sizes[i] + chunk - 1) // chunk
-        struct.pack_into("QQqii" * len(ids), a, 0, *row)
-        a.count, a.ptype, a.gtype, a.bits = len(ids), _TYPES[t], _TYPES[gt], bits
+        table = rows.copy()
+        table["p"], table["g"] = (pp, gp) if ids is None else (pp[ids], gp[ids])
+        C.memmove(C.addressof(a), table.__array_interface__["data"][0], table.nbytes)
+        a.count, a.ptype, a.gtype, a.bits = len(table), pt, gt, bits
         a.m, a.v = state["exp_avg"].data_ptr(), state["exp_avg_sq"].data_ptr()
         if bits == 8:
             a.m_scale, a.v_scale = state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()
@@ -363,18 +389,17 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
         calls.append(a)
     calls[-1].last = 1
     from . import ops
-    guard = ops._SCHED_STATUS.get(dev.index)
-    with _On(dev) as stream:
+    guard = ops._SCHED_STATUS.get(index)
+    if clip > 0:
+        slots = L.ADAMW_NORM_SLOTS // len(calls)
+        if slots == 0:
+            _fail(f"adamw_step: clipping over more than {L.ADAMW_NORM_SLOTS * L.ADAMW_MAX} tensors")
+        part = params[0].new_empty(L.ADAMW_NORM_SLOTS, dtype=torch.float64)
+        for k, a in enumerate(calls):
+            _launch(lib.sb_adamw_norm, dev, a, part.data_ptr(), k * slots, slots)
+    for a in calls:
         if clip > 0:
-            slots = L.ADAMW_NORM_SLOTS // len(calls)
-            if slots == 0:
-                _fail(f"adamw_step: clipping over more than {L.ADAMW_NORM_SLOTS * L.ADAMW_MAX} tensors")
-            part = torch.empty(L.ADAMW_NORM_SLOTS, dtype=torch.float64, device=dev)
-            for k, a in enumerate(calls):
-                L.check(lib.sb_adamw_norm(a, part.data_ptr(), k * slots, slots, stream), "sb_adamw_norm")
-        for a in calls:
-            if clip > 0:
-                a.norm_part, a.norm_slots = part.data_ptr(), slots * len(calls)
-            if guard is not None:
-                a.guard, a.skipped = guard.data_ptr(), _ptr(skipped)
-            L.check(lib.sb_adamw_step(a, stream), "sb_adamw_step")
+            a.norm_part, a.norm_slots = part.data_ptr(), slots * len(calls)
+        if guard is not None:
+            a.guard, a.skipped = guard.data_ptr(), _ptr(skipped)
+        _launch(lib.sb_adamw_step, dev, a)
