@@ -10,6 +10,13 @@ from . import _lib as L
 from . import ops_seq
 
 
+def _once_differentiable(backward):
+    """torch's once_differentiable where somebody asks for a graph of the gradients, nothing around the call where nobody does (a
+    backward pass of a small operator is its Python calls)"""
+    checked = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *grads: (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+
 class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -19,12 +26,11 @@ class LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        _, need_w, need_b, _ = ctx.needs_input_grad
-        dx, dw, db = ops_seq.layer_norm_bwd(dy, x, weight, mean, rstd, need_w, need_b, ctx.wdtype)
-        return dx if ctx.needs_input_grad[0] else None, dw, db, None
+        need = ctx.needs_input_grad
+        dx, dw, db = ops_seq.layer_norm_bwd(dy, *ctx.saved_tensors, need[1], need[2], ctx.wdtype, check=False)
+        return dx if need[0] else None, dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -45,7 +51,7 @@ class GatedScanFn(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, dh, dlast):
         x, gate, states, lengths = ctx.saved_tensors
         if dh is None and dlast is None:

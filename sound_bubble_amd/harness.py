@@ -20,7 +20,7 @@ import numpy as np
 import torch
 
 from .metrics import batch_metrics
-from .train import FlatBucket, FusedAdam, allreduce_grads, broadcast_replica
+from .train import FlatBucket, FusedAdam, FusedAdamW, allreduce_grads, broadcast_replica
 
 ALIASES = {
     "src.models.tfgridnet_realtime_clean_dis_embd3.net.Net": "sound_bubble_amd.net.NetDisEmbd3",
@@ -75,11 +75,13 @@ class PLModule(object):
         self.loss_fn = import_attr(loss)(**(loss_params or {}))
         if init_ckpt is not None:
             self.model.load_state_dict(load_model_weights(init_ckpt))
-        if optimizer not in ("torch.optim.Adam",):
-            raise NotImplementedError(f"optimizer {optimizer}: only torch.optim.Adam (every shipped config) is fused")
+        fused = {"torch.optim.Adam": FusedAdam, "torch.optim.AdamW": FusedAdamW}
+        if optimizer not in fused:
+            raise NotImplementedError(f"optimizer {optimizer}: only torch.optim.Adam (every shipped config) and torch.optim.AdamW "
+                                      "(optimizer_params may hold state_bits: 8) are fused")
         self.optim_name, self.opt_params = optimizer, dict(optimizer_params)
         self.bucket = FlatBucket(self.model)
-        self.optimizer = FusedAdam(self.bucket, **self.opt_params)
+        self.optimizer = fused[optimizer](self.bucket, **self.opt_params)
         self.grad_clip = grad_clip
         if self.grad_clip is None:
             print("NOT USING GRAD CLIP (pl_module_args.grad_clip is unset -- as in syn_experiments/pretrain_stage.json)")

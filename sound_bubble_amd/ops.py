@@ -2115,5 +2115,5 @@ def lstm_gen_bwd(dirs, rec, dhs, u, hs, geom, targets):
 
 
 # ---- sequence-block operators (include/sound_bubble_seq.h) ----
-from .ops_seq import (adamw_blocks, adamw_state, adamw_step, gated_scan_bwd, gated_scan_fwd, gated_scan_step,  # noqa: E402,F401
-                      layer_norm_bwd, layer_norm_fwd)
+from .ops_seq import (adamw_blocks, adamw_state, adamw_state_pack, adamw_state_values, adamw_step,  # noqa: E402,F401
+                      gated_scan_bwd, gated_scan_fwd, gated_scan_step, layer_norm_bwd, layer_norm_fwd)

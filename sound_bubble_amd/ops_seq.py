@@ -86,7 +86,7 @@ def layer_norm_fwd(x, weight, bias, eps=1e-5, stats=True):
     y = _like(x)
     mean = rstd = None
     if stats:
-        mean, rstd = x.new_empty((2,) + x.shape[:-1], dtype=torch.float32).unbind(0)
+        mean, rstd = (x.new_empty(x.shape[:-1], dtype=torch.float32) for _ in range(2))
     rows = x.numel() // n
     if rows == 0:
         return y, mean, rstd
@@ -99,15 +99,19 @@ def layer_norm_fwd(x, weight, bias, eps=1e-5, stats=True):
     return y, mean, rstd
 
 
-def layer_norm_bwd(dy, x, weight, mean, rstd, want_dw=True, want_db=True, wdtype=None):
+def layer_norm_bwd(dy, x, weight, mean, rstd, want_dw=True, want_db=True, wdtype=None, check=True):
     """-> (dx, dw, db) of layer_norm_fwd; dw / db (None where not wanted) in `wdtype` (the weight's, or given for a bias alone),
     summed over the rows in float32 in an order that the shape alone fixes"""
-    _need(x, "layer_norm_bwd: x", _TYPES)
-    n = _norm_params(x, weight, None)
-    _need(dy, "layer_norm_bwd: dy", (x.dtype,), x.device, x.shape)
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if not _need(t, f"layer_norm_bwd: {name}", (torch.float32,), x.device, x.shape[:-1]).is_contiguous():
-            _fail(f"layer_norm_bwd: {name} must be contiguous")
+    if check:      # (False: they are layer_norm_fwd's own, and autograd has seen to dy)
+        _need(x, "layer_norm_bwd: x", _TYPES)
+        _norm_params(x, weight, None)
+        _need(dy, "layer_norm_bwd: dy", (x.dtype,), x.device, x.shape)
+        for t, name in ((mean, "mean"), (rstd, "rstd")):
+            if not _need(t, f"layer_norm_bwd: {name}", (torch.float32,), x.device, x.shape[:-1]).is_contiguous():
+                _fail(f"layer_norm_bwd: {name} must be contiguous")
+        if wdtype is not None and wdtype not in (x.dtype, torch.float32):
+            _fail(f"layer_norm_bwd: wdtype is {x.dtype} or float32, got {wdtype}")
+    n = x.shape[-1]
     wdtype = weight.dtype if weight is not None else (wdtype or x.dtype)
     dx = _like(x)
     dw = x.new_empty(n, dtype=wdtype) if want_dw else None
@@ -269,6 +273,41 @@ def adamw_state(params, bits=32):
         for p, b in zip(params, starts):
             st["master"][b * L.ADAMW_BLOCK:b * L.ADAMW_BLOCK + p.numel()].copy_(p.detach().reshape(-1))
     return st
+
+
+_EIGHT = {"exp_avg": (torch.float8_e4m3fn, 448.0), "exp_avg_sq": (torch.float8_e5m2, 57344.0)}
+
+
+def adamw_state_values(state):
+    """the float32 values that adamw_step's states stand for (exact): {"exp_avg", "exp_avg_sq"}"""
+    out = {}
+    for k in _EIGHT:
+        v = state[k]
+        out[k] = v if v.dtype == torch.float32 else (v.float().view(-1, L.ADAMW_BLOCK) * state[k + "_scale"].float()[:, None]).view(-1)
+    return out
+
+
+def adamw_state_pack(state, values):
+    """`values` (float32 of the buffers' length) into `state`; where that has 8 bits each is rounded to the nearest code, values of
+    adamw_state_values come back exactly, and no positive exp_avg_sq becomes 0"""
+    for k, (kind, largest) in _EIGHT.items():
+        x = values[k]
+        if state[k].dtype == torch.float32:
+            state[k].copy_(x)
+            continue
+        x = x.float().view(-1, L.ADAMW_BLOCK)
+        big = x.abs().amax(1)
+        man, exp = torch.frexp(big / largest)                    # big <= largest * 2^e, e the smallest
+        e = torch.where(man == 0.5, exp - 1, exp).clamp(-127, 127)
+        e = torch.where(big == 0, -127, e)
+        byte = torch.where(torch.isfinite(big), e + 127, 255).to(torch.uint8)
+        scale = byte.view(torch.float8_e8m0fnu).float()[:, None]
+        y = torch.where(torch.isfinite(big)[:, None], x / scale, 0.0)
+        code = y.clamp(-largest, largest).to(kind).view(torch.uint8)
+        if k == "exp_avg_sq":
+            code = torch.where((code == 0) & (x > 0), 1, code)
+        state[k].view(torch.uint8).copy_(code.reshape(-1))
+        state[k + "_scale"].view(torch.uint8).copy_(byte)
 
 
 _ROW = np.dtype([("p", "u8"), ("g", "u8"), ("n", "i8"), ("first_block", "i4"), ("first_chunk", "i4")])      # sb_adamw_tensor

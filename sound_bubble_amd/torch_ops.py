@@ -15,6 +15,11 @@ separator as ONE opaque node per call:
   sound_bubble::snrlp_loss(est, gt, neg_weight) -> (loss, loss_vec, d_est)          -- SNRLP.py:17-42
   sound_bubble::multireso_fuse_loss(est, gt, cfg) -> (loss, d_est)                  -- MultiResoLoss.py:6-31
 
+and the sequence-block operators, one node each (functional_seq.py has them without the dispatcher):
+  sound_bubble::layer_norm(x, weight?, bias?, eps) -> (y, mean, rstd)
+  sound_bubble::gated_scan(x, gate, h0?, lengths?, dim, form, reverse) -> (h, last, states)
+  sound_bubble::gated_scan_step(x, gate, state(mutated), form) -> y
+
 Why one operator for the separator and not one per stage: the stage functions (functional.py) hand each other kernel-private
 state that is not a tensor in the dispatcher's sense -- BPTT records in tile-blocked layouts, the overlapped schedules'
 slab flags (`ops.FwdOverlap`), the FiLM bank every block's backward adds into, gradient targets inside the flat bucket --
@@ -35,6 +40,7 @@ import torch
 from torch import Tensor
 
 from . import functional as Fn
+from . import ops_seq
 from .streaming import flatten_state, unflatten_state_buffers
 
 _MODELS = weakref.WeakValueDictionary()     # model id -> Net (the operator's `model` argument)
@@ -382,6 +388,117 @@ def _mr_bwd(ctx, g_loss, g_d):
 
 
 multireso_fuse_loss.register_autograd(_mr_bwd, setup_context=_mr_setup)
+
+
+# ---- sequence-block operators ----
+@torch.library.custom_op("sound_bubble::layer_norm", mutates_args=(), device_types="cuda")
+def layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """(y, mean, rstd) of functional.layer_norm"""
+    return ops_seq.layer_norm_fwd(x, weight, bias, eps)
+
+
+@layer_norm.register_fake
+def _(x, weight, bias, eps):
+    return (torch.empty_like(x, memory_format=torch.contiguous_format), x.new_empty(x.shape[:-1], dtype=torch.float32),
+            x.new_empty(x.shape[:-1], dtype=torch.float32))
+
+
+@torch.library.custom_op("sound_bubble::layer_norm_backward", mutates_args=(), device_types="cuda")
+def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], mean: Tensor, rstd: Tensor, want_w: bool, want_b: bool,
+                        bias_f32: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    dx, dw, db = ops_seq.layer_norm_bwd(dy, x, weight, mean, rstd, want_w, want_b, torch.float32 if bias_f32 else x.dtype)
+    return dx, x.new_empty(0) if dw is None else dw, x.new_empty(0) if db is None else db
+
+
+@layer_norm_backward.register_fake
+def _(dy, x, weight, mean, rstd, want_w, want_b, bias_f32):
+    wt = weight.dtype if weight is not None else torch.float32 if bias_f32 else x.dtype
+    n = x.shape[-1]
+    return (torch.empty_like(x, memory_format=torch.contiguous_format), x.new_empty(n, dtype=wt) if want_w else x.new_empty(0),
+            x.new_empty(n, dtype=wt) if want_b else x.new_empty(0))
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    x, weight, bias, _ = inputs
+    ctx.save_for_backward(x, weight, output[1], output[2])
+    ctx.bias_f32 = bias is not None and bias.dtype == torch.float32
+    ctx.set_materialize_grads(False)
+
+
+def _layer_norm_bwd(ctx, dy, d_mean, d_rstd):
+    if d_mean is not None or d_rstd is not None:
+        raise RuntimeError("sound_bubble::layer_norm: mean and rstd have no gradient")
+    if dy is None:
+        return None, None, None, None
+    x, weight, mean, rstd = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx, dw, db = torch.ops.sound_bubble.layer_norm_backward(dy, x, weight, mean, rstd, need[1], need[2], ctx.bias_f32)
+    return dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None
+
+
+layer_norm.register_autograd(_layer_norm_bwd, setup_context=_layer_norm_setup)
+
+
+@torch.library.custom_op("sound_bubble::gated_scan", mutates_args=(), device_types="cuda")
+def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor], lengths: Optional[Tensor], dim: int, form: str,
+               reverse: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """(h, last, the states its backward pass starts from) of functional.gated_scan"""
+    return ops_seq.gated_scan_fwd(x, gate, h0, dim=dim, form=form, reverse=reverse, lengths=lengths)
+
+
+def _rest(x, dim):
+    dim = dim % x.dim()
+    return x.shape[:dim] + x.shape[dim + 1:]
+
+
+@gated_scan.register_fake
+def _(x, gate, h0, lengths, dim, form, reverse):
+    d = dim % x.dim()
+    outer, inner = x.shape[:d].numel(), x.shape[d + 1:].numel()
+    chunks = ops_seq._scan_plan(int(outer), int(x.shape[d]), int(inner), ops_seq._TYPES[x.dtype])[0]
+    return (torch.empty_like(x, memory_format=torch.contiguous_format), x.new_empty(_rest(x, dim), dtype=torch.float32),
+            x.new_empty(chunks * outer * inner, dtype=torch.float32))
+
+
+@torch.library.custom_op("sound_bubble::gated_scan_backward", mutates_args=(), device_types="cuda")
+def gated_scan_backward(dh: Optional[Tensor], dlast: Optional[Tensor], x: Tensor, gate: Tensor, states: Tensor, lengths: Optional[Tensor],
+                        dim: int, form: str, reverse: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    return ops_seq.gated_scan_bwd(dh, dlast, x, gate, states, dim=dim, form=form, reverse=reverse, lengths=lengths)
+
+
+@gated_scan_backward.register_fake
+def _(dh, dlast, x, gate, states, lengths, dim, form, reverse):
+    return (torch.empty_like(x, memory_format=torch.contiguous_format), torch.empty_like(gate, memory_format=torch.contiguous_format),
+            x.new_empty(_rest(x, dim), dtype=torch.float32))
+
+
+def _gated_scan_setup(ctx, inputs, output):
+    x, gate, _, lengths, ctx.dim, ctx.form, ctx.reverse = inputs
+    ctx.save_for_backward(x, gate, output[2], lengths)
+    ctx.set_materialize_grads(False)
+
+
+def _gated_scan_bwd(ctx, dh, dlast, d_states):
+    if d_states is not None:
+        raise RuntimeError("sound_bubble::gated_scan: the kept states have no gradient")
+    if dh is None and dlast is None:
+        return (None,) * 7
+    x, gate, states, lengths = ctx.saved_tensors
+    got = torch.ops.sound_bubble.gated_scan_backward(dh, dlast, x, gate, states, lengths, ctx.dim, ctx.form, ctx.reverse)
+    return tuple(g if need else None for g, need in zip(got, ctx.needs_input_grad)) + (None,) * 4
+
+
+gated_scan.register_autograd(_gated_scan_bwd, setup_context=_gated_scan_setup)
+
+
+@torch.library.custom_op("sound_bubble::gated_scan_step", mutates_args=("state",), device_types="cuda")
+def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor, form: str) -> Tensor:
+    return ops_seq.gated_scan_step(x, gate, state, form=form)
+
+
+@gated_scan_step.register_fake
+def _(x, gate, state, form):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 class _SeparateModule(torch.nn.Module):

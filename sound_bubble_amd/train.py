@@ -68,6 +68,10 @@ class FusedAdam:
                       gscale=1.0 / world_size, clip=clip, sumsq_buf=self.sumsq, skipped=self.skipped)
         bump_weight_epoch()       # the kernel wrote the parameters behind torch's version counters: weight forms are stale
 
+    def state_tensors(self):
+        """what makes two replicas' optimisers the same, beside step_count and lr (broadcast_replica)"""
+        return [self.m, self.v]
+
     def state_dict(self):
         """torch.optim.Adam.state_dict() layout (what the reference's dump_state stores under 'optimizer',
         hl_module:141-156): per-parameter {step, exp_avg, exp_avg_sq} indexed in model.parameters() order, sliced out of
@@ -122,6 +126,127 @@ class FusedAdam:
         self.betas, self.eps = tuple(g0.get("betas", self.betas)), g0.get("eps", self.eps)
 
 
+class FusedAdamW:
+    """torch.optim.AdamW(lr, betas, eps, weight_decay) semantics (no amsgrad) over a FlatBucket or any list of parameters -- float32,
+    or bfloat16 / float16 with an fp32 master copy -- in one launch for 112 tensors (ops.adamw_step), with
+    clip_grad_norm_(max_norm=grad_clip) folded in.
+
+    state_bits = 8 keeps exp_avg and exp_avg_sq as 8-bit floats with a power-of-two scale for every 256 elements: 2 bytes a parameter
+    instead of 8; `seed` is their rounding's.  A parameter whose .grad is None is left alone in that step.
+    capturable = True keeps step and lr on the device, so that a captured step counts on at every replay; `lr` is then taken over
+    from param_groups by every step outside a capture, or by sync_lr()."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False, state_bits=32, seed=0,
+                 capturable=False):
+        if amsgrad:
+            raise NotImplementedError("amsgrad is not used by any shipped config")
+        self.params = list(params.params if isinstance(params, FlatBucket) else params)
+        if not self.params:
+            raise ValueError("FusedAdamW: no parameters")
+        self.lr, self.betas, self.eps, self.weight_decay, self.seed = lr, tuple(betas), eps, weight_decay, int(seed)
+        self.state = ops.adamw_state(self.params, state_bits)
+        self.starts = [b * ops.L.ADAMW_BLOCK for b in ops.adamw_blocks([p.numel() for p in self.params])]
+        dev = self.params[0].device
+        self.capturable = bool(capturable)
+        self._step = torch.zeros(1, dtype=torch.int32, device=dev) if capturable else 0
+        self._lr_dev = torch.full((1,), float(lr), dtype=torch.float32, device=dev) if capturable else None
+        self.skipped = torch.zeros(1, device=dev, dtype=torch.int32)       # as FusedAdam's
+        self.param_groups = [{"lr": lr}]
+
+    @property
+    def step_count(self):
+        """(synchronises where capturable)"""
+        return int(self._step)
+
+    @step_count.setter
+    def step_count(self, n):
+        if self.capturable:
+            self._step.fill_(int(n))
+        else:
+            self._step = int(n)
+
+    def sync_lr(self):
+        """param_groups' lr to the device, for graphs that are replayed"""
+        if self.capturable:
+            self._lr_dev.fill_(float(self.param_groups[0]["lr"]))
+
+    def step(self, grad_clip=None, world_size=1):
+        """grads already SUMMED over ranks; they are scaled by 1/world_size here."""
+        if self.capturable:
+            if not torch.cuda.is_current_stream_capturing():
+                self.sync_lr()
+            self._step.add_(1)
+            step, lr = self._step, self._lr_dev
+        else:
+            step, lr = self._step + 1, self.param_groups[0]["lr"]
+        with torch.no_grad():
+            ops.adamw_step(self.params, [p.grad for p in self.params], self.state, step, lr=lr, betas=self.betas, eps=self.eps,
+                           weight_decay=self.weight_decay, gscale=1.0 / world_size, clip=float(grad_clip) if grad_clip else 0.0,
+                           seed=self.seed, skipped=self.skipped)
+        if not self.capturable:
+            self._step = step
+        torch.autograd.graph.increment_version(self.params)      # the kernel wrote them behind torch's version counters
+        bump_weight_epoch()
+
+    def zero_grad(self, set_to_none=True):
+        for p in self.params:
+            if p.grad is not None:
+                if set_to_none and not getattr(p, "_sb_flat_grad", False):
+                    p.grad = None
+                else:
+                    p.grad.zero_()
+
+    def state_tensors(self):
+        return [t if t.dtype == torch.float32 else t.view(torch.uint8) for t in self.state.values()]
+
+    def state_dict(self):
+        """torch.optim.AdamW.state_dict() layout, as FusedAdam's; 8-bit states as the float32 values they stand for, and
+        `master_param` for a 16-bit parameter"""
+        state, n = {}, self.step_count
+        if n > 0:
+            values = ops.adamw_state_values(self.state)
+            if "master" in self.state:
+                values["master_param"] = self.state["master"]
+            for i, (p, o) in enumerate(zip(self.params, self.starts)):
+                state[i] = {"step": torch.tensor(float(n)), **{k: v[o:o + p.numel()].view(p.shape).clone() for k, v in values.items()
+                                                               if k != "master_param" or p.dtype != torch.float32}}
+        group = {"lr": self.param_groups[0]["lr"], "betas": self.betas, "eps": self.eps, "weight_decay": self.weight_decay,
+                 "amsgrad": False, "maximize": False, "foreach": None, "capturable": self.capturable, "differentiable": False,
+                 "fused": None, "decoupled_weight_decay": True, "params": list(range(len(self.params)))}
+        return {"state": state, "param_groups": [group]}
+
+    def load_state_dict(self, sd):
+        """torch.optim.AdamW's layout; the states keep this optimiser's number of bits"""
+        groups = sd["param_groups"]
+        order = [i for g in groups for i in g["params"]]
+        if len(order) != len(self.params):
+            raise ValueError(f"optimizer state covers {len(order)} parameters, the model has {len(self.params)}")
+        g0 = groups[0]
+        if g0.get("amsgrad", False) or g0.get("maximize", False):
+            raise NotImplementedError("amsgrad / maximize optimizer states are not supported")
+        values = {k: torch.zeros_like(v) for k, v in ops.adamw_state_values(self.state).items()}
+        steps = set()
+        for slot, p, o in zip(order, self.params, self.starts):
+            st, n = sd["state"].get(slot), p.numel()
+            if "master" in self.state:
+                self.state["master"][o:o + n].copy_((st or {}).get("master_param", p.detach()).reshape(-1))
+            if st is None:
+                continue
+            if tuple(st["exp_avg"].shape) != tuple(p.shape):
+                raise ValueError(f"optimizer state {slot}: shape {tuple(st['exp_avg'].shape)} != parameter {tuple(p.shape)}")
+            for k in values:
+                values[k][o:o + n].copy_(st[k].reshape(-1))
+            steps.add(int(float(st["step"])))
+        if len(steps) > 1:
+            raise ValueError(f"per-parameter AdamW step counts differ ({sorted(steps)}): one shared step is supported")
+        ops.adamw_state_pack(self.state, values)
+        self.step_count = steps.pop() if steps else 0
+        self.param_groups[0]["lr"] = g0["lr"]
+        self.sync_lr()
+        self.betas, self.eps = tuple(g0.get("betas", self.betas)), g0.get("eps", self.eps)
+        self.weight_decay = g0.get("weight_decay", self.weight_decay)
+
+
 def _via_host(t):
     """gloo (CPU tests; several ranks on one GPU in the -m gpu tests) moves device tensors through the host"""
     import torch.distributed as dist
@@ -148,8 +273,8 @@ def broadcast_replica(bucket, optim=None, src=0):
     _broadcast(bucket.flat, src)
     bump_weight_epoch()
     if optim is not None:
-        _broadcast(optim.m, src)
-        _broadcast(optim.v, src)
+        for t in optim.state_tensors():
+            _broadcast(t, src)
         meta = torch.tensor([float(optim.step_count), float(optim.param_groups[0]["lr"])], device=bucket.flat.device,
                             dtype=torch.float64)
         _broadcast(meta, src)

@@ -119,3 +119,86 @@ def test_adamw_layout():
     from sound_bubble_amd import ops
     assert ops.adamw_blocks([]) == [0]
     assert ops.adamw_blocks([1, 256, 257, 0, 5]) == [0, 1, 2, 4, 4, 5]
+
+
+def test_fake_implementations_propagate_shapes(torch_mod):
+    torch = torch_mod
+    from sound_bubble_amd import torch_ops  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    sb = torch.ops.sound_bubble
+    with FakeTensorMode():
+        x = torch.empty(3, 300, 40, device="cuda", dtype=torch.bfloat16)
+        w = torch.empty(40, device="cuda")
+        y, mean, rstd = sb.layer_norm(x, w, None, 1e-5)
+        assert y.shape == x.shape and y.dtype == x.dtype and mean.shape == rstd.shape == (3, 300) and mean.dtype == torch.float32
+        dx, dw, db = sb.layer_norm_backward(y, x, w, mean, rstd, True, False, False)
+        assert dx.shape == x.shape and dw.shape == (40,) and dw.dtype == torch.float32 and db.shape == (0,)
+        h, last, states = sb.gated_scan(x, x, None, None, 1, "sigmoid", False)
+        assert h.shape == x.shape and last.shape == (3, 40) and last.dtype == states.dtype == torch.float32 and states.numel() % 120 == 0
+        dx, dg, d0 = sb.gated_scan_backward(h, None, x, x, states, None, 1, "sigmoid", False)
+        assert dx.shape == dg.shape == x.shape and d0.shape == (3, 40)
+        assert sb.gated_scan_step(x[:, 0], x[:, 0], last, "decay").shape == (3, 40)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        sb.layer_norm(torch.zeros(2, 3), None, None, 1e-5)
+
+
+def test_adamw_states_pack_exactly(torch_mod):
+    """8-bit states -> float32 -> 8-bit states keeps every value; a value is rounded to the nearest code"""
+    torch = torch_mod
+    from sound_bubble_amd import ops_seq as Q
+    g = torch.Generator().manual_seed(1)
+    st = {}
+    for k, (kind, _) in Q._EIGHT.items():
+        top = 0x7F if kind is torch.float8_e4m3fn else 0x7C
+        code = torch.randint(0, top, (2048,), generator=g, dtype=torch.uint8)
+        if k == "exp_avg":
+            code |= torch.randint(0, 2, (2048,), generator=g, dtype=torch.uint8) << 7
+        code[256:512] = 0
+        st[k] = code.view(kind)
+        st[k + "_scale"] = torch.randint(60, 180, (8,), generator=g, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    st["exp_avg"].view(torch.uint8)[512:768] = 0x01                     # a block of the smallest code only: another scale, the same values
+    want = Q.adamw_state_values(st)
+    two = {k: torch.zeros_like(v.view(torch.uint8)).view(v.dtype) for k, v in st.items()}
+    Q.adamw_state_pack(two, want)
+    got = Q.adamw_state_values(two)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    x = {"exp_avg": torch.randn(2048, generator=g), "exp_avg_sq": torch.randn(2048, generator=g).square()}
+    x["exp_avg_sq"][5] = 1e-30
+    x["exp_avg"][300] = float("inf")
+    Q.adamw_state_pack(two, x)
+    got = Q.adamw_state_values(two)
+    assert got["exp_avg_sq"][5] > 0 and torch.isnan(got["exp_avg"][256:512]).all()
+    fine = torch.ones(2048, dtype=torch.bool)
+    fine[256:512] = False
+    for k, half in (("exp_avg", 2.0 ** -4), ("exp_avg_sq", 2.0 ** -3)):
+        low = x[k][fine].abs().max() * (2.0 ** -17 if k == "exp_avg" else 2.0 ** -30)      # half the smallest code, at most
+        assert ((got[k] - x[k]).abs()[fine] <= x[k].abs()[fine] * half + low).all()
+
+
+def test_replicas_share_the_optimiser_state(torch_mod, tmp_path):
+    """broadcast_replica moves whatever state_tensors() names (two ranks over gloo; FusedAdam's moments here)"""
+    torch = torch_mod
+    import subprocess
+    import sys
+    src = tmp_path / "rank.py"
+    src.write_text("""
+import sys, torch, torch.distributed as dist
+sys.path.insert(0, %r)
+from sound_bubble_amd.train import broadcast_replica
+rank = int(sys.argv[1])
+dist.init_process_group("gloo", init_method="tcp://127.0.0.1:%%s" %% sys.argv[2], rank=rank, world_size=2)
+class Bucket: flat = torch.full((4,), float(rank))
+class Optim:
+    step_count, param_groups = 3 + rank, [{"lr": 0.5 + rank}]
+    codes = torch.full((5,), 7 + rank, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    def state_tensors(self): return [self.codes.view(torch.uint8)]
+o = Optim()
+broadcast_replica(Bucket, o)
+assert Bucket.flat.eq(0).all() and o.codes.view(torch.uint8).eq(7).all() and o.step_count == 3 and o.param_groups[0]["lr"] == 0.5
+""" % ROOT)
+    import socket
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = str(s.getsockname()[1])
+    procs = [subprocess.Popen([sys.executable, str(src), str(r), port]) for r in range(2)]
+    assert [p.wait(timeout=120) for p in procs] == [0, 0]
