@@ -1,4 +1,5 @@
-"""Build libsoundbubble_hip.so (gfx950) in-tree with hipcc.  No torch dependency."""
+"""Build libsoundbubble_hip.so (gfx950) in-tree with hipcc -- no torch dependency -- and, beside it, libsoundbubble_torch.so: the
+sequence-block operators' calls from PyTorch (csrc/seq/sb_seq_torch.cpp), host code against the headers of the torch that is installed."""
 import os
 import subprocess
 import sys
@@ -16,6 +17,23 @@ HEADERS = [os.path.join(CSRC, "sb_common.h"), os.path.join(CSRC, "sb_lstm_bf_com
            os.path.join(HERE, "..", "include", "sound_bubble_hip.h")]
 SEQ_HEADERS = [os.path.join(CSRC, "sb_common.h"), os.path.join(CSRC, "seq", "sb_seq_common.h"),
                os.path.join(HERE, "..", "include", "sound_bubble_seq.h")]
+
+
+TORCH_LIB = os.path.join(LIBDIR, "libsoundbubble_torch.so")
+TORCH_SOURCE = os.path.join(CSRC, "seq", "sb_seq_torch.cpp")
+
+
+def torch_lib_cmd():
+    """the compiler line of libsoundbubble_torch.so (torch is looked up, not imported)"""
+    import importlib.util
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("libsoundbubble_torch.so needs an installed torch")
+    t = spec.submodule_search_locations[0]
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-D_GLIBCXX_USE_CXX11_ABI=1",
+            "-I" + os.path.join(t, "include"), "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(rocm, "include"),
+            TORCH_SOURCE, "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch"]
 
 
 def csrc_digest():
@@ -77,6 +95,8 @@ def build(force=False, verbose=True):
             cmd[2:2] = os.environ.get("SB_EXTRA_HIPCC_FLAGS", "").split()
             cmd[2:2] = flags
             jobs.append(cmd)
+    if force or _stale(TORCH_LIB, [TORCH_SOURCE, SEQ_HEADERS[-1]]):
+        jobs.append(torch_lib_cmd())
     if jobs:                                   # translation units are independent: compile them side by side
         from concurrent.futures import ThreadPoolExecutor
 

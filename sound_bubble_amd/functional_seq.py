@@ -10,6 +10,22 @@ from . import _lib as L
 from . import ops_seq
 
 
+def _native(name, *args):
+    """the call without Python in between, where it is one of the plain ones; empty: not taken, the wrappers see to it or say what is
+    wrong"""
+    native = ops_seq.native()
+    if native is None:
+        return ()
+    try:
+        return getattr(native, name)(*args)
+    except (RuntimeError, TypeError):
+        return ()
+
+
+def _recorded(*tensors):
+    return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)
+
+
 def _once_differentiable(backward):
     """torch's once_differentiable where somebody asks for a graph of the gradients, nothing around the call where nobody does (a
     backward pass of a small operator is its Python calls)"""
@@ -36,7 +52,10 @@ class LayerNormFn(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis, in x's type; weight / bias of shape (n,) in x's type or
     float32"""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    out = _native("layer_norm", x, weight, bias, eps)
+    if out:
+        return out[0]
+    if _recorded(x, weight, bias):
         return LayerNormFn.apply(x, weight, bias, eps)
     return ops_seq.layer_norm_fwd(x, weight, bias, eps, stats=False)[0]
 
@@ -70,7 +89,10 @@ def gated_scan(x, gate, h0=None, *, dim=1, form="sigmoid", reverse=False, length
     lengths (int64 / int32, x.shape[:dim]): a padded batch; steps at and behind a sequence's length leave its state alone, their
     outputs and gradients are 0 and their inputs are not looked at.
     x and gate may be halves of one projection: a dense last axis is enough, other layouts are copied."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, h0)):
+    out = _native("gated_scan", x, gate, h0, lengths, dim, ops_seq.FORMS.get(form, -1), reverse)
+    if out:
+        return tuple(out)
+    if _recorded(x, gate, h0):
         return GatedScanFn.apply(x, gate, h0, lengths, dim, form, reverse)
     return ops_seq.gated_scan_fwd(x, gate, h0, dim=dim, form=form, reverse=reverse, lengths=lengths, save=False)[:2]
 
@@ -78,7 +100,10 @@ def gated_scan(x, gate, h0=None, *, dim=1, form="sigmoid", reverse=False, length
 def gated_scan_step(x, gate, state, *, form="sigmoid"):
     """One step of gated_scan for streaming: state (float32, x's shape, dense) is updated in place; -> its value in x's type.  No
     gradients: gated_scan with one step has them."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate, state)):
+    out = _native("gated_scan_step", x, gate, state, ops_seq.FORMS.get(form, -1))
+    if out:
+        return out[0]
+    if _recorded(x, gate, state):
         raise L.SoundBubbleHipError("gated_scan_step updates the state in place and has no gradient: call gated_scan, or this under "
                                     "torch.no_grad()")
     return ops_seq.gated_scan_step(x, gate, state, form=form)

@@ -2115,5 +2115,8 @@ def lstm_gen_bwd(dirs, rec, dhs, u, hs, geom, targets):
 
 
 # ---- sequence-block operators (include/sound_bubble_seq.h) ----
+from . import ops_seq as _ops_seq  # noqa: E402
 from .ops_seq import (adamw_blocks, adamw_state, adamw_state_pack, adamw_state_values, adamw_step,  # noqa: E402,F401
                       gated_scan_bwd, gated_scan_fwd, gated_scan_step, layer_norm_bwd, layer_norm_fwd)
+
+_ops_seq._OPS = __import__("sys").modules[__name__]

@@ -7,11 +7,14 @@ stream of the tensors' own device; what a call needs besides its results is allo
 import ctypes as C
 import functools
 import itertools
+import os
 
 import numpy as np
 import torch
 
 from . import _lib as L
+
+_OPS = None         # the module ops, which imports this one (it sets the name)
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 FORMS = {"decay": 0, "sigmoid": 1}
@@ -21,10 +24,41 @@ def _fail(msg):
     raise L.SoundBubbleHipError(msg)
 
 
+_NATIVE = None      # the operators of libsoundbubble_torch.so, False: there is no such library
+
+
+class _Native:
+    def __init__(self):
+        lib = L.load()
+        ops = torch.ops.sound_bubble_seq
+        ops.bind([C.cast(getattr(lib, name), C.c_void_p).value for name in _ENTRIES])
+        self.layer_norm, self.gated_scan = ops.layer_norm.default, ops.gated_scan.default
+        self.gated_scan_step, self.adamw_step = ops.gated_scan_step.default, ops.adamw_step.default
+
+
+_ENTRIES = ("sb_layer_norm_fwd", "sb_layer_norm_bwd_scratch", "sb_layer_norm_bwd", "sb_gated_scan_plan", "sb_gated_scan_fwd", "sb_gated_scan_bwd",
+            "sb_gated_scan_step", "sb_adamw_chunk", "sb_adamw_norm", "sb_adamw_step")      # csrc/seq/sb_seq_torch.cpp: Entries
+
+
+def native():
+    """The plain calls without Python in between (csrc/seq/sb_seq_torch.cpp): same kernels, same results, a fraction of the host time.
+    They answer with an empty list (0) what they do not take; None where the library has not been built, or inside ops.on_stream."""
+    global _NATIVE
+    if _NATIVE is None:
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsoundbubble_torch.so")
+        _NATIVE = False
+        if os.path.exists(path) and os.environ.get("SB_SEQ_HOST", "") != "python":
+            torch.ops.load_library(path)
+            _NATIVE = _Native()
+    return _NATIVE if _NATIVE and _OPS._STREAM_OVERRIDE is None else None
+
+
 def _need(t, name, dtypes, device=None, shape=None):
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.layout is torch.strided):
         _fail(f"{name}: expected a tensor of {' / '.join(str(d)[6:] for d in dtypes)} on the GPU, got "
               f"{type(t).__name__} {getattr(t, 'dtype', '')} {getattr(t, 'device', '')}")
+    if t.is_neg():
+        _fail(f"{name}: a lazily negated tensor (call .resolve_neg())")
     if device is not None and t.device != device:
         _fail(f"{name}: is on {t.device}, the call's tensors are on {device}")
     if shape is not None and tuple(t.shape) != tuple(shape):
@@ -38,12 +72,11 @@ def _ptr(t):
 
 def _launch(fn, device, *args):
     """fn(*args, stream) on the tensors' own device and its current stream (ops.on_stream's, inside one)"""
-    from . import ops
     index = device.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _launch(fn, device, *args)
-    stream = ops._STREAM_OVERRIDE
+    stream = _OPS._STREAM_OVERRIDE
     if stream is None:
         stream = torch._C._cuda_getCurrentRawStream(index)
     rc = fn(*args, stream)
@@ -238,6 +271,8 @@ def gated_scan_step(x, gate, state, *, form="sigmoid"):
         return y
     n = x.shape[-1] if x.dim() else 1
     (xr, ldx), (gr, ldg) = _rows(x, n), _rows(gate, n)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     _launch(L.load().sb_gated_scan_step, x.device, xr.data_ptr(), gr.data_ptr(), state.data_ptr(), y.data_ptr(), x.numel() // n, n, ldx, ldg,
             _TYPES[x.dtype], _TYPES[gate.dtype], FORMS[form])
     return y
@@ -360,6 +395,26 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
     tensors.  seed: of the 8-bit states' rounding.  skipped: counts a step that the device's watchdog word turned into a no-op
     (ops.adam_step)."""
     params, grads = list(params), list(grads)
+    step_dev = lr_dev = None
+    if isinstance(step, torch.Tensor):
+        step_dev, step = step, 0
+    elif params and getattr(params[0], "is_cuda", False) and torch.cuda.is_current_stream_capturing():
+        _fail("adamw_step: a captured graph would repeat this step's number at every replay: pass step as an int32 tensor")
+    if isinstance(lr, torch.Tensor):
+        lr_dev, lr = lr, 0.0
+    fast = native()
+    if fast is not None and params and isinstance(state.get("exp_avg"), torch.Tensor):
+        bits = 8 if state["exp_avg"].dtype == torch.float8_e4m3fn else 32
+        keys = ["exp_avg", "exp_avg_sq"] + ["exp_avg_scale", "exp_avg_sq_scale"] * (bits == 8) + ["master"] * (params[0].dtype != torch.float32)
+        guard = _OPS._SCHED_STATUS.get(params[0].get_device())
+        try:
+            done = fast.adamw_step(params, grads, [state[k] for k in keys], bits, step, step_dev, lr, lr_dev, *betas, eps, weight_decay, gscale, clip,
+                                   seed & 0xFFFFFFFF, guard.data_ptr() if guard is not None else 0,
+                                   skipped.data_ptr() if guard is not None and skipped is not None else 0)
+        except (RuntimeError, TypeError, KeyError):      # (what it is, is said below)
+            done = 0
+        if done:
+            return
     if len(params) != len(grads):
         _fail(f"adamw_step: {len(params)} parameters, {len(grads)} gradients")
     if not params:
@@ -391,19 +446,13 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
     bits = _adamw_check_state(state, blocks, dev, need_master)
     if blocks >= 1 << 31:
         _fail("adamw_step: more than 2^31 blocks of states")
-    step_dev = lr_dev = None
-    if isinstance(step, torch.Tensor):
-        step_dev, step = _need(step, "adamw_step: step", (torch.int32,), dev), 0
-        if step_dev.numel() != 1:
+    if step_dev is not None:
+        if _need(step_dev, "adamw_step: step", (torch.int32,), dev).numel() != 1:
             _fail("adamw_step: step is one number")
     elif step < 1 or step >= 1 << 31:
         _fail(f"adamw_step: step counts from 1, got {step}")
-    elif torch.cuda.is_current_stream_capturing():
-        _fail("adamw_step: a captured graph would repeat this step's number at every replay: pass step as an int32 tensor")
-    if isinstance(lr, torch.Tensor):
-        lr_dev, lr = _need(lr, "adamw_step: lr", (torch.float32,), dev), 0.0
-        if lr_dev.numel() != 1:
-            _fail("adamw_step: lr is one number")
+    if lr_dev is not None and _need(lr_dev, "adamw_step: lr", (torch.float32,), dev).numel() != 1:
+        _fail("adamw_step: lr is one number")
     if clip < 0:
         _fail(f"adamw_step: clip is a norm (0: none), got {clip}")
     if not batches:
@@ -427,8 +476,8 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
         a.gscale, a.clip = gscale, clip
         calls.append(a)
     calls[-1].last = 1
-    from . import ops
-    guard = ops._SCHED_STATUS.get(index)
+    guard = _OPS._SCHED_STATUS.get(index)
+    torch.autograd.graph.increment_version(ps)
     if clip > 0:
         slots = L.ADAMW_NORM_SLOTS // len(calls)
         if slots == 0:

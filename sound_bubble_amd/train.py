@@ -185,7 +185,6 @@ class FusedAdamW:
                            seed=self.seed, skipped=self.skipped)
         if not self.capturable:
             self._step = step
-        torch.autograd.graph.increment_version(self.params)      # the kernel wrote them behind torch's version counters
         bump_weight_epoch()
 
     def zero_grad(self, set_to_none=True):

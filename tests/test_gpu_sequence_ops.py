@@ -729,3 +729,67 @@ def test_two_graphs_do_not_share_memory(torch_mod):
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1])
+
+
+def test_calls_with_and_without_python_in_between(torch_mod, monkeypatch):
+    """the library's own calls (csrc/seq/sb_seq_torch.cpp) and the Python wrappers: the same bits, refusals and version counts"""
+    torch = torch_mod
+    from sound_bubble_amd import functional as F, ops, ops_seq
+    assert ops_seq.native() is not None
+    ins = scan_inputs(torch, (3, 200, 24), 1, torch.bfloat16, torch.float32, "sigmoid", 97, ragged=True)
+
+    def everything():
+        x, gate, h0, lengths, dh, dlast = ins
+        out = []
+        for t in (x, x.transpose(0, 1), x[:, ::2]):
+            w = torch.ones(24, device="cuda", requires_grad=True)
+            leaf = t.detach().requires_grad_(True)
+            y = F.layer_norm(leaf, w, w.detach())
+            out += [y.detach(), *torch.autograd.grad(y, (leaf, w), t)]
+        for rev in (False, True):
+            leaves = [t.detach().requires_grad_(True) for t in (x, gate, h0)]
+            h, last = F.gated_scan(*leaves, lengths=lengths.int(), reverse=rev)
+            out += [h.detach(), last.detach(), *torch.autograd.grad((h, last), leaves, (dh, dlast))]
+        out += F.gated_scan(x, gate, dim=-1, form="decay")
+        state = h0.clone()
+        v = state._version
+        out += [F.gated_scan_step(x[:, 0], gate[:, 0], state), state]
+        assert state._version == v + 1
+        for bits, dt in ((32, torch.float32), (8, torch.bfloat16)):
+            g = gen(torch, 3)
+            ps = [torch.randn(n, generator=g, device="cuda").to(dt) for n in [5] * 130 + [70000]]
+            st = ops.adamw_state(ps, bits)
+            v = ps[0]._version
+            for step in (1, 2):
+                ops.adamw_step(ps, [p.clone() for p in ps], st, step, lr=1e-2, clip=0.5, seed=9)
+            assert ps[0]._version == v + 2
+            out += ps + [t.view(torch.uint8) for t in st.values()]
+        return out
+    a = everything()
+    monkeypatch.setattr(ops_seq, "_NATIVE", False)
+    b = everything()
+    assert len(a) == len(b) and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_refusals_without_the_native_calls(torch_mod, monkeypatch):
+    from sound_bubble_amd import ops_seq
+    monkeypatch.setattr(ops_seq, "_NATIVE", False)
+    test_refusals(torch_mod)
+    test_gated_scan_layouts(torch_mod)
+    test_layer_norm_layouts(torch_mod)
+    test_adamw_skips_and_order(torch_mod)
+
+
+def test_more_refusals(torch_mod):
+    """lazily negated and sparse tensors, a state that is no buffer of its own, gradients through the step"""
+    torch = torch_mod
+    from sound_bubble_amd import functional as F
+    from sound_bubble_amd._lib import SoundBubbleHipError as E
+    neg = torch.randn(4, 8, dtype=torch.complex64, device="cuda").conj().imag
+    assert neg.is_neg()
+    h = torch.zeros(4, 8, device="cuda")
+    leaf = h.clone().requires_grad_(True)
+    for call in (lambda: F.layer_norm(neg), lambda: F.gated_scan(h, neg), lambda: F.layer_norm(h.to_sparse()), lambda: F.gated_scan_step(h, h, neg),
+                 lambda: F.gated_scan_step(leaf, h, h), lambda: F.gated_scan_step(h, h, h.t().contiguous().t()), lambda: F.layer_norm([1.0])):
+        with pytest.raises(E):
+            call()
