@@ -33,7 +33,7 @@ def torch_lib_cmd():
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-D_GLIBCXX_USE_CXX11_ABI=1",
             "-I" + os.path.join(t, "include"), "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(rocm, "include"),
-            TORCH_SOURCE, "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch"]
+            TORCH_SOURCE, "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-lamdhip64", "-ltorch_cpu", "-ltorch"]
 
 
 def csrc_digest():

@@ -11,6 +11,8 @@
 // The backward pass makes h_{t-1} again in fp32 from the states the forward pass left in front of every chunk, and walks
 //   G_t = dh_t + c_{t+1},  c_t = a_t G_t
 // down the same chunks: the pairs are (A, D): c -> A c + D, with A the forward pass's product.
+#include <cmath>
+
 #include "sb_seq_common.h"
 
 namespace {
@@ -20,7 +22,9 @@ namespace {
 constexpr int S = 16, kMaxWaves = 8;
 // Workgroups with fewer waves than kFewWaves in all leave the chip half empty: time is cut so that there are about kWaves.  That reads x and
 // gate twice.  fp16 6 x 3001 x 1000 (752 waves) forward / backward, us: cut 68 / 94, whole 94 / 134.
-constexpr int kFewWaves = 1024, kWaves = 4096, kMaxSplits = 64;
+// A segment joins the pairs of all in front of it, 0.1 us each, and walks its own chunks, 2.4 us each in both kernels: of c chunks about
+// 5 sqrt(c) segments.  fp32 1 x 262144 x 16 forward / backward, us: 64 segments 217 / 258, 226 87 / 106; 1 x 65536 x 64: 64 49 / 56, 113 40 / 45.
+constexpr int kFewWaves = 1024, kWaves = 4096, kMaxSplits = 512;
 
 struct Lay {
   int nw, splits;                  // waves along time, segments of time
@@ -38,7 +42,10 @@ Lay lay_of(int64_t outer, int64_t steps, int64_t inner) {
   l.chunks = (steps + l.steps - 1) / l.steps;
   l.splits = 1;
   const int64_t waves = l.tiles * l.nw;
-  if (waves < kFewWaves && l.chunks >= 4) l.splits = (int)std::min<int64_t>(std::min<int64_t>(kMaxSplits, l.chunks / 2), (kWaves + waves - 1) / waves);
+  if (waves < kFewWaves && l.chunks >= 4) {
+    const int64_t most = std::min<int64_t>(kMaxSplits, std::min<int64_t>(l.chunks / 2, (int64_t)(5 * std::sqrt((double)l.chunks))));
+    l.splits = (int)std::min<int64_t>(most, (kWaves + waves - 1) / waves);
+  }
   return l;
 }
 

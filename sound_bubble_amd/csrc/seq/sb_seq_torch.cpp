@@ -7,8 +7,10 @@
 // from there too (bind), so that one library serves both.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -68,6 +70,21 @@ struct NoSecond : torch::autograd::Function<NoSecond> {
 };
 Tensor once(const Tensor& value, const Tensor& through) {
   return value.defined() && at::GradMode::is_enabled() && through.defined() && through.requires_grad() ? NoSecond::apply(value, through) : value;
+}
+
+// A leaf that an eager graph still holds has its gradient's node on that graph's stream; a backward pass under capture would wait for that stream,
+// which ends the capture and the process.  Said here, in the forward call under capture.
+void refuse_held_leaves(std::initializer_list<const Tensor*> leaves, const Tensor& like) {
+  const c10::OptionalDeviceGuard guard(like.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto id = c10::hip::getCurrentHIPStream(like.device().index()).id();
+  for (const Tensor* t : leaves) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream || stream->id() == id, "sound_bubble: an eager graph of this leaf, made on another stream, is alive while a graph is captured: "
+                "drop it (its outputs and losses) before the capture");
+  }
 }
 
 // ---- layer norm ----
@@ -143,8 +160,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 std::vector<Tensor> layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps) {
   if (!norm_takes(x, weight, bias)) return {};
-  if (at::GradMode::is_enabled() && (x.requires_grad() || (given(weight) && weight->requires_grad()) || (given(bias) && bias->requires_grad())))
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (given(weight) && weight->requires_grad()) || (given(bias) && bias->requires_grad()))) {
+    const Tensor w = or_none(weight), b = or_none(bias);
+    refuse_held_leaves({&x, &w, &b}, x);
     return {LayerNorm::apply(x, weight, bias, eps)};
+  }
   return {norm_fwd(x, or_none(weight), or_none(bias), eps, nullptr, nullptr)};
 }
 
@@ -265,8 +285,11 @@ std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const Maybe&
     lengths = lengths_->to(at::kLong).contiguous();
   }
   const Sizes z = sizes_of(x, dim);
-  if (at::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || (given(h0) && h0->requires_grad())))
+  if (at::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || (given(h0) && h0->requires_grad()))) {
+    const Tensor first = or_none(h0);
+    refuse_held_leaves({&x, &gate, &first}, x);
     return GatedScan::apply(x, gate, h0, lengths, z.dim, form, reverse);
+  }
   const auto [h, last] = scan_fwd(x, gate, or_none(h0), or_none(lengths), z, form, reverse, nullptr);
   return {h, last};
 }
@@ -305,6 +328,12 @@ int64_t adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>&
       return 0;
     blocks += (p.numel() + SB_ADAMW_BLOCK - 1) / SB_ADAMW_BLOCK;
   }
+  std::vector<const void*> places(count);
+  for (size_t i = 0; i < count; ++i) places[i] = params[i].data_ptr();
+  std::sort(places.begin(), places.end());
+  if (std::adjacent_find(places.begin(), places.end()) != places.end()) return 0;
+  const auto rate = [](double v) { return v >= 0 && v < 1; };
+  if (!rate(beta1) || !rate(beta2) || !(eps >= 0)) return 0;
   const size_t buffers = (bits == 8 ? 4 : 2) + (ptype != at::kFloat);
   const size_t slots_per = SB_ADAMW_NORM_SLOTS / ((count + SB_ADAMW_MAX - 1) / SB_ADAMW_MAX);
   if ((bits != 8 && bits != 32) || state.size() != buffers || blocks >= (1LL << 31) || slots_per == 0 || !(clip >= 0)) return 0;

@@ -18,7 +18,9 @@ def _native(name, *args):
         return ()
     try:
         return getattr(native, name)(*args)
-    except (RuntimeError, TypeError):
+    except (RuntimeError, TypeError) as e:
+        if str(e).startswith("sound_bubble:"):
+            raise L.SoundBubbleHipError(str(e)) from None
         return ()
 
 

@@ -453,7 +453,11 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
         _fail(f"adamw_step: step counts from 1, got {step}")
     if lr_dev is not None and _need(lr_dev, "adamw_step: lr", (torch.float32,), dev).numel() != 1:
         _fail("adamw_step: lr is one number")
-    if clip < 0:
+    if not all(0 <= b < 1 for b in betas) or not eps >= 0:
+        _fail(f"adamw_step: betas are in [0, 1) and eps is not negative, got {betas}, {eps}")
+    if len({p.data_ptr() for p, n in zip(params, sizes) if n}) < sum(n > 0 for n in sizes):
+        _fail("adamw_step: a parameter is given twice")
+    if not clip >= 0:
         _fail(f"adamw_step: clip is a norm (0: none), got {clip}")
     if not batches:
         return

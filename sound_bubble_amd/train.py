@@ -133,6 +133,7 @@ class FusedAdamW:
 
     state_bits = 8 keeps exp_avg and exp_avg_sq as 8-bit floats with a power-of-two scale for every 256 elements: 2 bytes a parameter
     instead of 8; `seed` is their rounding's.  A parameter whose .grad is None is left alone in that step.
+    16-bit parameters that something else has written (a checkpoint, say) are taken over into the master copy by sync_master().
     capturable = True keeps step and lr on the device, so that a captured step counts on at every replay; `lr` is then taken over
     from param_groups by every step outside a capture, or by sync_lr()."""
 
@@ -164,6 +165,12 @@ class FusedAdamW:
             self._step.fill_(int(n))
         else:
             self._step = int(n)
+
+    def sync_master(self):
+        """the parameters' present values to their fp32 master copies"""
+        if "master" in self.state:
+            for p, o in zip(self.params, self.starts):
+                self.state["master"][o:o + p.numel()].copy_(p.detach().reshape(-1))
 
     def sync_lr(self):
         """param_groups' lr to the device, for graphs that are replayed"""

@@ -793,3 +793,53 @@ def test_more_refusals(torch_mod):
                  lambda: F.gated_scan_step(leaf, h, h), lambda: F.gated_scan_step(h, h, h.t().contiguous().t()), lambda: F.layer_norm([1.0])):
         with pytest.raises(E):
             call()
+
+
+def test_adamw_refuses_what_it_cannot_mean(torch_mod):
+    torch = torch_mod
+    from sound_bubble_amd import ops
+    from sound_bubble_amd._lib import SoundBubbleHipError as E
+    p = torch.ones(300, device="cuda")
+    two = [p, torch.ones(20, device="cuda"), p]
+    st = ops.adamw_state(two)
+    with pytest.raises(E, match="twice"):
+        ops.adamw_step(two, two, st, 1, lr=0.1)
+    one = ops.adamw_state([p])
+    for kw in (dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1.0), dict(eps=float("nan")), dict(clip=float("nan"))):
+        with pytest.raises(E):
+            ops.adamw_step([p], [p], one, 1, lr=0.1, **kw)
+    assert p.eq(1).all()
+
+
+def test_capture_refuses_leaves_of_a_live_eager_graph(torch_mod):
+    """the forward call under capture says so (its backward pass would end the process); without the eager graph it goes on"""
+    torch = torch_mod
+    from sound_bubble_amd import functional as F
+    from sound_bubble_amd._lib import SoundBubbleHipError as E
+    x = torch.randn(4, 50, 16, device="cuda")
+    w = torch.ones(16, device="cuda", requires_grad=True)
+    z = torch.zeros(4, 50, 16, device="cuda", requires_grad=True)
+    eager = F.layer_norm(x, w), F.gated_scan(x, z)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        try:
+            for call in (lambda: F.layer_norm(x, w), lambda: F.gated_scan(x, z)):
+                with pytest.raises(E, match="eager graph"):
+                    call()
+            keep = x + 1
+        finally:
+            graph.capture_end()
+    torch.cuda.current_stream().wait_stream(s)
+    del eager, keep
+    want = torch.autograd.grad(F.layer_norm(x, w).sum() + F.gated_scan(x, z)[0].sum(), (w, z))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(F.layer_norm(x, w).sum() + F.gated_scan(x, z)[0].sum(), (w, z))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        F.layer_norm(x)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
