@@ -44,7 +44,7 @@ Lay lay_of(int64_t outer, int64_t steps, int64_t inner) {
   const int64_t waves = l.tiles * l.nw;
   if (waves < kFewWaves && l.chunks >= 4) {
     const int64_t most = std::min<int64_t>(kMaxSplits, std::min<int64_t>(l.chunks / 2, (int64_t)(5 * std::sqrt((double)l.chunks))));
-    l.splits = (int)std::min<int64_t>(most, (kWaves + waves - 1) / waves);
+    l.splits = (int)std::min<int64_t>(most, kWaves / waves);
   }
   return l;
 }
@@ -219,15 +219,83 @@ template <bool UP> SB_DEVINL float fold_splits(const float* start, const Place& 
   return carry;
 }
 
-// MODE 0: h, states, h_last.  MODE 1: the pair of segment blockIdx.y into agg.
-template <class T, class G, int FORM, int MODE>
+// The pair of a segment of time: (A, B) of blockIdx.y from x and gate (UP), (A, D) of blockIdx.y + 1 from dh and gate.  The waves take
+// consecutive parts of it, each by itself, and are joined once.
+template <class T, class G, int FORM, bool UP>
+__global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_pair_kernel(Kargs k) {
+  extern __shared__ float2 lds[];
+  const Place p(k);
+  const Pairs pairs{lds, p.waves};
+  const int split = blockIdx.y + (UP ? 0 : 1);
+  const int64_t g0 = k.chunks * split / k.splits * p.waves, groups = k.chunks * (split + 1) / k.splits * p.waves - g0;
+  const int64_t first = (g0 + groups * p.wave / p.waves) * S, last = (g0 + groups * (p.wave + 1) / p.waves) * S - S;      // (>= one group a wave)
+  const void* from = UP ? k.x : k.dh;
+  const int64_t so = UP ? k.so_x : k.so_d, st = UP ? k.st_x : k.st_d, step = UP ? S : -S;
+  float carry = 0.f, whole = 1.f;
+  T x[S];
+  G g[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) x[s] = (T)0.f;
+  const auto load = [&](int64_t t, bool full) __attribute__((always_inline)) {
+    const unsigned live = full ? 0u : p.live(t);
+    load_steps<G>(g, k.gate, k.so_g, k.st_g, p, k, t, full, live);
+    if (full || from) load_steps<T>(x, from, so, st, p, k, t, full, live);
+  };
+  const auto group = [&](int64_t t, auto fast, bool more) __attribute__((always_inline)) {
+    constexpr bool FAST = decltype(fast)::value;
+    float a[S], ol[S], xf[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      a[s] = (float)g[s];
+      xf[s] = (float)x[s];      // (dead steps were loaded as 0)
+    }
+    const bool full = FAST || p.full(t);
+    const unsigned live = full ? 0u : p.live(t);
+    if constexpr (FAST) load(t + step, true);
+    else if (more) load(t + step, from && p.full(t + step));
+#pragma unroll
+    for (int s = 0; s < S; ++s) coefficients<FORM>(a[s], a[s], ol[s]);
+    if (!full) kill_dead(a, ol, live);
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const int s = UP ? i : S - 1 - i;
+      whole *= a[s];
+      carry = UP ? __builtin_fmaf(a[s], carry, ol[s] * xf[s]) : a[s] * (xf[s] + carry);
+    }
+  };
+  int64_t t = UP ? first : last;
+  int64_t left = (last - first) / S + 1;
+  load(t, from && p.full(t));
+  for (; left > 0; --left, t += step) {
+    wait_memory();
+    if (from)
+      for (; left > 1 && p.full(t) && p.full(t + step); --left, t += step) group(t, std::true_type(), true);
+    group(t, std::false_type(), left > 1);
+  }
+  if (p.waves > 1) {
+    pairs.at(0, p.wave) = make_float2(whole, carry);
+    block_sync();
+    float in;
+    carry = 0.f;
+    pairs.template join<UP>(0, -1, carry, in);
+    whole = pairs.product(0);
+  }
+  if (p.wave == 0 && p.on) {
+    const int64_t plane = k.outer * k.inner;
+    k.agg[(2 * split) * plane + p.q] = whole;
+    k.agg[(2 * split + 1) * plane + p.q] = carry;
+  }
+}
+
+// h, states, h_last
+template <class T, class G, int FORM>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(Kargs k) {
   extern __shared__ float2 lds[];
   const Place p(k);
   const Pairs pairs{lds, p.waves};
   const int split = blockIdx.y;
   const int64_t c0 = k.chunks * split / k.splits, c1 = k.chunks * (split + 1) / k.splits, plane = k.outer * k.inner;
-  float carry = MODE == 0 ? fold_splits<true>(k.h0, p, k, split) : 0.f, whole = 1.f;
+  float carry = fold_splits<true>(k.h0, p, k, split);
   T x[S];
   G g[S];
   const auto load = [&](int64_t t, bool full) __attribute__((always_inline)) {
@@ -260,28 +328,24 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(Kargs k)
       A = s ? A * a[s] : a[s];
       B = s ? __builtin_fmaf(a[s], B, b[s]) : b[s];
     }
-    if (MODE == 0 && k.states && p.wave == 0 && p.on) k.states[ch * plane + p.q] = carry;
+    if (k.states && p.wave == 0 && p.on) k.states[ch * plane + p.q] = carry;
     float in;
     if (p.waves > 1) {
       pairs.at(ch & 1, p.wave) = make_float2(A, B);
       block_sync();
-      if constexpr (MODE == 1) whole *= pairs.product(ch & 1);
       pairs.template join<true>(ch & 1, p.wave, carry, in);
     } else {
       in = carry;
       carry = __builtin_fmaf(A, carry, B);
-      if constexpr (MODE == 1) whole *= A;
     }
-    if constexpr (MODE == 0) {
-      T out[S];
+    T out[S];
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        in = __builtin_fmaf(a[s], in, b[s]);
-        out[s] = (T)in;
-      }
-      if (!full) kill_dead<T>(out, live);
-      store_steps<T>(k.h, out, p, k, t, full);
+    for (int s = 0; s < S; ++s) {
+      in = __builtin_fmaf(a[s], in, b[s]);
+      out[s] = (T)in;
     }
+    if (!full) kill_dead<T>(out, live);
+    store_steps<T>(k.h, out, p, k, t, full);
   };
   load(start(c0), p.full(start(c0)));
   for (int64_t ch = c0; ch < c1; ++ch) {
@@ -289,25 +353,18 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(Kargs k)
     for (; ch + 1 < c1 && p.full(start(ch)) && p.full(start(ch + 1)); ++ch) chunk(ch, std::true_type());
     chunk(ch, std::false_type());
   }
-  if (p.wave == 0 && p.on) {
-    if constexpr (MODE == 0) {
-      if (split == k.splits - 1) k.h_last[p.q] = carry;
-    } else {
-      k.agg[(2 * split) * plane + p.q] = whole;
-      k.agg[(2 * split + 1) * plane + p.q] = carry;
-    }
-  }
+  if (p.wave == 0 && p.on && split == k.splits - 1) k.h_last[p.q] = carry;
 }
 
-// MODE 0: dx, dgate, dh0.  MODE 1: the pair (A, D) of segment blockIdx.y + 1 into agg.
-template <class T, class G, int FORM, int MODE>
+// dx, dgate, dh0
+template <class T, class G, int FORM>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(Kargs k) {
   extern __shared__ float2 lds[];
   const Place p(k);
   const Pairs down{lds, p.waves}, up{lds + 2 * 64 * p.waves, p.waves};
-  const int split = blockIdx.y + (MODE == 1 ? 1 : 0);
+  const int split = blockIdx.y;
   const int64_t c0 = k.chunks * split / k.splits, c1 = k.chunks * (split + 1) / k.splits, plane = k.outer * k.inner;
-  float carry = MODE == 0 ? fold_splits<false>(k.dlast, p, k, split) : 0.f, whole = 1.f;
+  float carry = fold_splits<false>(k.dlast, p, k, split);
   T x[S], d[S];
   G g[S];
   float state = 0.f;
@@ -317,10 +374,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(Kargs k)
     const unsigned live = full ? 0u : p.live(t);
     load_steps<G>(g, k.gate, k.so_g, k.st_g, p, k, t, full, live);
     if (has) load_steps<T>(d, k.dh, k.so_d, k.st_d, p, k, t, full, live);
-    if constexpr (MODE == 0) {
-      load_steps<T>(x, k.x, k.so_x, k.st_x, p, k, t, full, live);
-      if (p.on) state = k.states[ch * plane + p.q];
-    }
+    load_steps<T>(x, k.x, k.so_x, k.st_x, p, k, t, full, live);
+    if (p.on) state = k.states[ch * plane + p.q];
   };
   const auto start = [&](int64_t ch) { return ch * k.chunk_steps + p.wave * S; };
   const auto chunk = [&](int64_t ch, auto fast) __attribute__((always_inline)) {
@@ -332,7 +387,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(Kargs k)
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       a[s] = (float)g[s];
-      xf[s] = MODE == 0 ? (float)x[s] : 0.f;      // (dead steps were loaded as 0)
+      xf[s] = (float)x[s];      // (dead steps were loaded as 0)
       df[s] = (float)d[s];
     }
     if constexpr (FAST) load(ch - 1, t - k.chunk_steps, true, true);
@@ -346,58 +401,49 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(Kargs k)
       A = s < S - 1 ? A * a[s] : a[s];
       D = a[s] * (s < S - 1 ? df[s] + D : df[s]);
     }
-    if constexpr (MODE == 0) {
 #pragma unroll
-      for (int s = 0; s < S; ++s) B = s ? __builtin_fmaf(a[s], B, ol[s] * xf[s]) : ol[0] * xf[0];
-    }
+    for (int s = 0; s < S; ++s) B = s ? __builtin_fmaf(a[s], B, ol[s] * xf[s]) : ol[0] * xf[0];
     float in;
     if (p.waves > 1) {
       down.at(ch & 1, p.wave) = make_float2(A, D);
-      if constexpr (MODE == 0) up.at(ch & 1, p.wave) = make_float2(A, B);
+      up.at(ch & 1, p.wave) = make_float2(A, B);
       block_sync();
-      if constexpr (MODE == 0) {
-        for (int w = 0; w < p.wave; ++w) {
-          const float2 r = up.at(ch & 1, w);
-          h = __builtin_fmaf(r.x, h, r.y);
-        }
-      } else {
-        whole *= down.product(ch & 1);
+      for (int w = 0; w < p.wave; ++w) {
+        const float2 r = up.at(ch & 1, w);
+        h = __builtin_fmaf(r.x, h, r.y);
       }
       down.template join<false>(ch & 1, p.wave, carry, in);
     } else {
       in = carry;
       carry = __builtin_fmaf(A, carry, D);
-      if constexpr (MODE == 1) whole *= A;
     }
-    if constexpr (MODE == 0) {
-      float hb[S];
+    float hb[S];
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        hb[s] = h;
-        h = __builtin_fmaf(a[s], h, ol[s] * xf[s]);
-      }
-      T dx[S];
-      G dg[S];
-#pragma unroll
-      for (int s = S - 1; s >= 0; --s) {
-        const float gt = df[s] + in;
-        in = a[s] * gt;
-        if constexpr (FORM == SB_SCAN_SIGMOID) {
-          const float vx = ol[s] * gt;
-          dx[s] = (T)vx;
-          dg[s] = (G)(vx * a[s] * (hb[s] - xf[s]));
-        } else {
-          dx[s] = (T)gt;
-          dg[s] = (G)(gt * hb[s]);
-        }
-      }
-      if (!full) {
-        kill_dead<T>(dx, live);
-        kill_dead<G>(dg, live);
-      }
-      store_steps<T>(k.dx, dx, p, k, t, full);
-      store_steps<G>(k.dgate, dg, p, k, t, full);
+    for (int s = 0; s < S; ++s) {
+      hb[s] = h;
+      h = __builtin_fmaf(a[s], h, ol[s] * xf[s]);
     }
+    T dx[S];
+    G dg[S];
+#pragma unroll
+    for (int s = S - 1; s >= 0; --s) {
+      const float gt = df[s] + in;
+      in = a[s] * gt;
+      if constexpr (FORM == SB_SCAN_SIGMOID) {
+        const float vx = ol[s] * gt;
+        dx[s] = (T)vx;
+        dg[s] = (G)(vx * a[s] * (hb[s] - xf[s]));
+      } else {
+        dx[s] = (T)gt;
+        dg[s] = (G)(gt * hb[s]);
+      }
+    }
+    if (!full) {
+      kill_dead<T>(dx, live);
+      kill_dead<G>(dg, live);
+    }
+    store_steps<T>(k.dx, dx, p, k, t, full);
+    store_steps<G>(k.dgate, dg, p, k, t, full);
   };
   load(c1 - 1, start(c1 - 1), p.full(start(c1 - 1)), k.dh != nullptr);
   for (int64_t ch = c1 - 1; ch >= c0; --ch) {
@@ -406,14 +452,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(Kargs k)
       for (; ch > c0 && p.full(start(ch)) && p.full(start(ch - 1)); --ch) chunk(ch, std::true_type());
     chunk(ch, std::false_type());
   }
-  if (p.wave == 0 && p.on) {
-    if constexpr (MODE == 0) {
-      if (split == 0 && k.dh0) k.dh0[p.q] = carry;
-    } else {
-      k.agg[(2 * split) * plane + p.q] = whole;
-      k.agg[(2 * split + 1) * plane + p.q] = carry;
-    }
-  }
+  if (p.wave == 0 && p.on && split == 0 && k.dh0) k.dh0[p.q] = carry;
 }
 
 template <class T, class G, int FORM>
@@ -498,8 +537,8 @@ extern "C" int sb_gated_scan_fwd(const sb_gated_scan_args* ap, void* stream) {
     const dim3 block(64 * l.nw);
     const unsigned lds = l.nw > 1 ? 16 * 64 * l.nw : 0;
     if (l.splits > 1)
-      hipLaunchKernelGGL((gated_scan_fwd_kernel<T, G, form.value, 1>), dim3((unsigned)l.tiles, l.splits - 1), block, lds, (hipStream_t)stream, k);
-    hipLaunchKernelGGL((gated_scan_fwd_kernel<T, G, form.value, 0>), dim3((unsigned)l.tiles, l.splits), block, lds, (hipStream_t)stream, k);
+      hipLaunchKernelGGL((gated_scan_pair_kernel<T, G, form.value, true>), dim3((unsigned)l.tiles, l.splits - 1), block, lds, (hipStream_t)stream, k);
+    hipLaunchKernelGGL((gated_scan_fwd_kernel<T, G, form.value>), dim3((unsigned)l.tiles, l.splits), block, lds, (hipStream_t)stream, k);
     SB_CHECK_LAUNCH();
     return 0;
   });
@@ -528,8 +567,8 @@ extern "C" int sb_gated_scan_bwd(const sb_gated_scan_bwd_args* ap, void* stream)
     const dim3 block(64 * l.nw);
     const unsigned lds = l.nw > 1 ? 32 * 64 * l.nw : 0;
     if (l.splits > 1)
-      hipLaunchKernelGGL((gated_scan_bwd_kernel<T, G, form.value, 1>), dim3((unsigned)l.tiles, l.splits - 1), block, lds, (hipStream_t)stream, k);
-    hipLaunchKernelGGL((gated_scan_bwd_kernel<T, G, form.value, 0>), dim3((unsigned)l.tiles, l.splits), block, lds, (hipStream_t)stream, k);
+      hipLaunchKernelGGL((gated_scan_pair_kernel<T, G, form.value, false>), dim3((unsigned)l.tiles, l.splits - 1), block, lds, (hipStream_t)stream, k);
+    hipLaunchKernelGGL((gated_scan_bwd_kernel<T, G, form.value>), dim3((unsigned)l.tiles, l.splits), block, lds, (hipStream_t)stream, k);
     SB_CHECK_LAUNCH();
     return 0;
   });
