@@ -257,7 +257,7 @@ def check_scan(torch, x, gate, h0, lengths, dh, dlast, **kw):
 
 SCAN_SHAPES = [((1, 1, 1), 1), ((2, 1, 64), 1), ((3, 7, 5), 1), ((2, 8, 8), 1), ((5, 65, 33), 1), ((2, 257, 130), 1), ((1, 1031, 3), 1), ((3, 300, 1), 1),
                ((4, 9, 6, 20), 1), ((4, 9, 37, 20), 2), ((70, 40, 9, 2), 2), ((33, 12, 145, 32), 2), ((5, 6), 1), ((9,), 0), ((600, 4, 7, 64), 2),
-               ((1, 5000, 16), 1), ((2, 3000, 200), 1)]
+               ((1, 5000, 16), 1), ((2, 3000, 200), 1), ((4, 700, 1501), 1), ((3, 130, 3001), 1), ((5, 20, 1000), 1), ((1500, 90, 3), 1)]
 
 
 @pytest.mark.parametrize("shape,dim", SCAN_SHAPES)
