@@ -65,7 +65,7 @@ void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with 
 struct NoSecond : torch::autograd::Function<NoSecond> {
   static Tensor forward(AutogradContext*, const Tensor& value, const Tensor&) { return value.alias(); }
   static variable_list backward(AutogradContext*, variable_list) {
-    TORCH_CHECK(false, "trying to differentiate twice a function that was marked with @once_differentiable");
+    TORCH_CHECK(false, "sound_bubble: layer_norm and gated_scan have no second derivative");
   }
 };
 Tensor once(const Tensor& value, const Tensor& through) {
