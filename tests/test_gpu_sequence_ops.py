@@ -385,8 +385,14 @@ def dither(n, step, seed):
     return x ^ (x >> 16)
 
 
-def encode(x, mant, bias, top, u16, floor):
-    """the 8-bit format's definition in integers of 64 bits and float64 (numpy): -> codes, scale bytes"""
+def inverses(torch):
+    """2^(127 - byte) as tensor operations give it on the device: for some exponents one ulp below the power of two"""
+    return torch.ldexp(torch.ones(256, device="cuda"), 127 - torch.arange(256, device="cuda", dtype=torch.int32)).cpu().numpy()
+
+
+def encode(x, inverse, mant, bias, top, u16, floor):
+    """the 8-bit format's definition in integers of 64 bits and float64 (numpy): -> codes, scale bytes.  inverse[byte]: what a
+    block is multiplied by before it is cut, in float32"""
     blocks = x.reshape(-1, 256).astype(np.float64)
     big = np.abs(blocks).max(1)
     largest = (2 - 0.25) * 2.0 ** top
@@ -394,7 +400,7 @@ def encode(x, mant, bias, top, u16, floor):
         k = np.where(big > 0, np.ceil(np.log2(np.maximum(big, 1e-300) / largest)), -127)
     k = np.where(big > 0, k + (big > largest * 2.0 ** k) - (big <= largest * 2.0 ** (k - 1)), k)      # (log2's own rounding)
     k = np.clip(k, -127, 127)
-    y = np.abs(blocks) / (2.0 ** k)[:, None]
+    y = (np.abs(blocks).astype(np.float32) * inverse[(k + 127).astype(int)][:, None]).astype(np.float64)
     e = np.maximum(np.floor(np.log2(np.maximum(y, 1e-300))), 1 - bias)
     unit = 2.0 ** (e - mant)                                          # spacing of the codes around y
     part = y / unit
@@ -489,12 +495,34 @@ def test_adamw_8(torch_mod, sizes, pt):
         m = m0 * f(b1) + gl * f(1 - b1)
         v = v0 * f(b2) + (gl * gl) * f(1 - b2)
         u = dither(m.size, step, 7).astype(np.int64)
-        mc, ms = encode(m, 3, 7, 8, u & 0xFFFF, False)
-        vc, vs = encode(v, 2, 15, 15, u >> 16, True)
+        mc, ms = encode(m, inverses(torch), 3, 7, 8, u & 0xFFFF, False)
+        vc, vs = encode(v, inverses(torch), 2, 15, 15, u >> 16, True)
         assert np.array_equal(st["exp_avg_scale"].view(torch.uint8).cpu().numpy(), ms)
         assert np.array_equal(st["exp_avg_sq_scale"].view(torch.uint8).cpu().numpy(), vs)
         assert np.array_equal(st["exp_avg"].view(torch.uint8).cpu().numpy(), mc)
         assert np.array_equal(st["exp_avg_sq"].view(torch.uint8).cpu().numpy(), vc)
+
+
+def test_adamw_8_scales(torch_mod):
+    """blocks of every magnitude, each of 16 mantissas of its largest element, and values that are a code's own: the definition's codes"""
+    torch = torch_mod
+    from sound_bubble_amd import ops
+    g = gen(torch, 44)
+    f, (b1, b2) = np.float32, HYPER["betas"]
+    unit = torch.arange(-60, 60, device="cuda").repeat_interleave(16)
+    blocks = unit.numel()
+    x = torch.randn(blocks, 256, generator=g, device="cuda") * torch.exp2(unit.float())[:, None]
+    x[:, 0] = torch.exp2(unit.float()) * (1 + torch.arange(blocks, device="cuda") % 16 / 16) * 4
+    x[:, 128:192] = torch.exp2(unit.float())[:, None] * torch.exp2(-torch.arange(64, device="cuda").float() / 8).round(decimals=2)
+    p = torch.zeros(blocks * 256, device="cuda")
+    st = ops.adamw_state([p], bits=8)
+    ops.adamw_step([p], [x.view(-1)], st, 1, seed=3, **HYPER)
+    gl = x.view(-1).cpu().numpy()
+    u = dither(gl.size, 1, 3).astype(np.int64)
+    for k, a, fmt, part in (("exp_avg", gl * f(1 - b1), (3, 7, 8), u & 0xFFFF), ("exp_avg_sq", (gl * gl) * f(1 - b2), (2, 15, 15), u >> 16)):
+        code, scale = encode(a, inverses(torch), *fmt, part, k == "exp_avg_sq")
+        assert np.array_equal(st[k + "_scale"].view(torch.uint8).cpu().numpy(), scale), k
+        assert np.array_equal(st[k].view(torch.uint8).cpu().numpy(), code), k
 
 
 def test_adamw_8_follows_a_falling_gradient(torch_mod):
