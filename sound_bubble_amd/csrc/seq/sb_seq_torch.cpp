@@ -74,7 +74,7 @@ Tensor once(const Tensor& value, const Tensor& through) {
 
 // A leaf that an eager graph still holds has its gradient's node on that graph's stream; a backward pass under capture would wait for that stream,
 // which ends the capture and the process.  Said here, in the forward call under capture.
-void refuse_held_leaves(std::initializer_list<const Tensor*> leaves, const Tensor& like) {
+void refuse_held_leaves(at::ArrayRef<const Tensor*> leaves, const Tensor& like) {
   const c10::OptionalDeviceGuard guard(like.device());
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   const auto id = c10::hip::getCurrentHIPStream(like.device().index()).id();
@@ -87,6 +87,14 @@ void refuse_held_leaves(std::initializer_list<const Tensor*> leaves, const Tenso
   }
 }
 
+void refuse_held(const std::vector<Tensor>& leaves) {
+  std::vector<const Tensor*> at;
+  for (const Tensor& t : leaves) at.push_back(&t);
+  if (!leaves.empty()) refuse_held_leaves(at, leaves[0]);
+}
+// forward-mode tangents are refused where autograd is: by the Python functions
+bool tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
 // ---- layer norm ----
 std::pair<Tensor, int64_t> rows_of(const Tensor& t, int64_t n) {
   if (t.is_contiguous()) return {t, n};
@@ -95,7 +103,7 @@ std::pair<Tensor, int64_t> rows_of(const Tensor& t, int64_t n) {
   return {r, r.size(0) > 1 ? r.stride(0) : n};
 }
 bool norm_takes(const Tensor& x, const Maybe& weight, const Maybe& bias) {
-  if (!plain(x) || x.dim() < 1 || x.numel() == 0) return false;
+  if (!plain(x) || x.dim() < 1 || x.numel() == 0 || tangent(x) || tangent(or_none(weight)) || tangent(or_none(bias))) return false;
   for (const Maybe* t : {&weight, &bias})
     if (given(*t) && (!plain(**t) || (*t)->device() != x.device() || (*t)->dim() != 1 || (*t)->size(0) != x.size(-1) ||
                       ((*t)->scalar_type() != x.scalar_type() && (*t)->scalar_type() != at::kFloat)))
@@ -198,7 +206,8 @@ Plan plan_of(const Sizes& z, const Tensor& x) {
 }
 bool scan_takes(const Tensor& x, const Tensor& gate, const Maybe& h0, const Maybe& lengths, int64_t dim, int64_t form) {
   if (!plain(x) || !plain(gate) || x.numel() == 0 || gate.device() != x.device() || gate.sizes() != x.sizes() || dim < -x.dim() || dim >= x.dim() ||
-      (gate.scalar_type() != x.scalar_type() && gate.scalar_type() != at::kFloat) || form < 0 || form > 1)
+      (gate.scalar_type() != x.scalar_type() && gate.scalar_type() != at::kFloat) || form < 0 || form > 1 || tangent(x) || tangent(gate) ||
+      tangent(or_none(h0)))
     return false;
   const Sizes z = sizes_of(x, dim);
   if (given(h0) && (!plain(*h0) || h0->scalar_type() != at::kFloat || h0->device() != x.device() || h0->sizes() != z.rest)) return false;
@@ -296,7 +305,7 @@ std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const Maybe&
 std::vector<Tensor> gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state, int64_t form) {
   if (!plain(x) || !plain(gate) || !plain(state) || x.numel() == 0 || x.dim() < 1 || gate.sizes() != x.sizes() || state.sizes() != x.sizes() ||
       gate.device() != x.device() || state.device() != x.device() || (gate.scalar_type() != x.scalar_type() && gate.scalar_type() != at::kFloat) ||
-      state.scalar_type() != at::kFloat || !state.is_contiguous() || form < 0 || form > 1 ||
+      state.scalar_type() != at::kFloat || !state.is_contiguous() || form < 0 || form > 1 || tangent(x) || tangent(gate) || tangent(state) ||
       (at::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || state.requires_grad())))
     return {};
   const c10::OptionalDeviceGuard guard(x.device());
@@ -398,6 +407,7 @@ int64_t adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>&
 
 TORCH_LIBRARY(sound_bubble_seq, m) {
   m.def("bind(int[] addresses) -> ()", bind);
+  m.def("refuse_held_leaves(Tensor[] leaves) -> ()", refuse_held);
   m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor[]", layer_norm);
   m.def("gated_scan(Tensor x, Tensor gate, Tensor? h0, Tensor? lengths, int dim, int form, bool reverse) -> Tensor[]", gated_scan);
   m.def("gated_scan_step(Tensor x, Tensor gate, Tensor(a!) state, int form) -> Tensor[]", gated_scan_step);

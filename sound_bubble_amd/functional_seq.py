@@ -25,6 +25,10 @@ def _native(name, *args):
 
 
 def _recorded(*tensors):
+    """whether autograd is concerned: with gradients, or with tangents (which the autograd functions refuse)"""
+    forward = torch.autograd.forward_ad
+    if forward._current_level >= 0 and any(forward.unpack_dual(t).tangent is not None for t in tensors if isinstance(t, torch.Tensor)):
+        return True
     return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)
 
 
@@ -47,7 +51,7 @@ class LayerNormFn(torch.autograd.Function):
     @_once_differentiable
     def backward(ctx, dy):
         need = ctx.needs_input_grad
-        dx, dw, db = ops_seq.layer_norm_bwd(dy, *ctx.saved_tensors, need[1], need[2], ctx.wdtype, check=False)
+        dx, dw, db = ops_seq.layer_norm_bwd(dy.resolve_neg(), *ctx.saved_tensors, need[1], need[2], ctx.wdtype, check=False)
         return dx if need[0] else None, dw, db, None
 
 
@@ -58,6 +62,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if out:
         return out[0]
     if _recorded(x, weight, bias):
+        ops_seq.refuse_held_leaves(x, weight, bias)
         return LayerNormFn.apply(x, weight, bias, eps)
     return ops_seq.layer_norm_fwd(x, weight, bias, eps, stats=False)[0]
 
@@ -78,6 +83,7 @@ class GatedScanFn(torch.autograd.Function):
         if dh is None and dlast is None:
             return (None,) * 7
         need = ctx.needs_input_grad
+        dh, dlast = (t if t is None else t.resolve_neg() for t in (dh, dlast))
         dx, dgate, dh0 = ops_seq.gated_scan_bwd(dh, dlast, x, gate, states, lengths=lengths, want_dh0=need[2], **ctx.how)
         return dx if need[0] else None, dgate if need[1] else None, dh0, None, None, None, None
 
@@ -89,12 +95,13 @@ def gated_scan(x, gate, h0=None, *, dim=1, form="sigmoid", reverse=False, length
     gates: with "decay" gates beyond 1 in magnitude, those products have to stay within float32.
     h0: float32, x's shape without `dim` (None: zeros).  reverse: from the last step to the first.
     lengths (int64 / int32, x.shape[:dim]): a padded batch; steps at and behind a sequence's length leave its state alone, their
-    outputs and gradients are 0 and their inputs are not looked at.
+    outputs and gradients are 0 and their inputs are not looked at (reverse: the walk begins at a sequence's last own step).
     x and gate may be halves of one projection: a dense last axis is enough, other layouts are copied."""
     out = _native("gated_scan", x, gate, h0, lengths, dim, ops_seq.FORMS.get(form, -1), reverse)
     if out:
         return tuple(out)
     if _recorded(x, gate, h0):
+        ops_seq.refuse_held_leaves(x, gate, h0)
         return GatedScanFn.apply(x, gate, h0, lengths, dim, form, reverse)
     return ops_seq.gated_scan_fwd(x, gate, h0, dim=dim, form=form, reverse=reverse, lengths=lengths, save=False)[:2]
 

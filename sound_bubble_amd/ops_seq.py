@@ -34,23 +34,42 @@ class _Native:
         ops.bind([C.cast(getattr(lib, name), C.c_void_p).value for name in _ENTRIES])
         self.layer_norm, self.gated_scan = ops.layer_norm.default, ops.gated_scan.default
         self.gated_scan_step, self.adamw_step = ops.gated_scan_step.default, ops.adamw_step.default
+        self.refuse_held_leaves = ops.refuse_held_leaves.default
 
 
 _ENTRIES = ("sb_layer_norm_fwd", "sb_layer_norm_bwd_scratch", "sb_layer_norm_bwd", "sb_gated_scan_plan", "sb_gated_scan_fwd", "sb_gated_scan_bwd",
             "sb_gated_scan_step", "sb_adamw_chunk", "sb_adamw_norm", "sb_adamw_step")      # csrc/seq/sb_seq_torch.cpp: Entries
+_PYTHON = os.environ.get("SB_SEQ_HOST", "") == "python"
 
 
-def native():
-    """The plain calls without Python in between (csrc/seq/sb_seq_torch.cpp): same kernels, same results, a fraction of the host time.
-    They answer with an empty list (0) what they do not take; None where the library has not been built, or inside ops.on_stream."""
+def _library():
     global _NATIVE
     if _NATIVE is None:
         path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsoundbubble_torch.so")
         _NATIVE = False
-        if os.path.exists(path) and os.environ.get("SB_SEQ_HOST", "") != "python":
+        if os.path.exists(path):
             torch.ops.load_library(path)
             _NATIVE = _Native()
-    return _NATIVE if _NATIVE and _OPS._STREAM_OVERRIDE is None else None
+    return _NATIVE
+
+
+def native():
+    """The plain calls without Python in between (csrc/seq/sb_seq_torch.cpp): same kernels, same results, a fraction of the host time.
+    They answer with an empty list (0) what they do not take; None where the library has not been built, with SB_SEQ_HOST=python, or
+    inside ops.on_stream."""
+    lib = _library()
+    return lib if lib and not _PYTHON and _OPS._STREAM_OVERRIDE is None else None
+
+
+def refuse_held_leaves(*leaves):
+    """Under capture: raises where an eager graph made on another stream holds one of the leaves (the captured backward pass would
+    wait for that stream, which ends the process)."""
+    leaves = [t for t in leaves if isinstance(t, torch.Tensor) and t.is_cuda and t.requires_grad]
+    if leaves and torch.cuda.is_current_stream_capturing() and _library():
+        try:
+            _library().refuse_held_leaves(leaves)
+        except RuntimeError as e:
+            raise L.SoundBubbleHipError(str(e)) from None
 
 
 def _need(t, name, dtypes, device=None, shape=None):
@@ -432,6 +451,10 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
         ps, gs, pts = [params[i] for i in take], [grads[i] for i in take], [ptypes[i] for i in take]
     else:
         take, ps, gs, pts = None, params, grads, ptypes
+    for i, g in enumerate(gs):
+        if g.layout is not torch.strided or g.is_neg():
+            what = "a lazily negated one (call .resolve_neg())" if g.layout is torch.strided else g.layout
+            _fail(f"adamw_step: gradient {take[i] if take else i}: expected a dense tensor, got {what}")
     gtypes = [g.dtype for g in gs]
     if {*map(T.get_device, gs)} - {index} or not all(map(T.is_same_size, ps, gs)) or \
             (gtypes != pts and any(a is not b and a is not torch.float32 for a, b in zip(gtypes, pts))):

@@ -420,6 +420,7 @@ def _(dy, x, weight, mean, rstd, want_w, want_b, bias_f32):
 
 def _layer_norm_setup(ctx, inputs, output):
     x, weight, bias, _ = inputs
+    ops_seq.refuse_held_leaves(x, weight, bias)
     ctx.save_for_backward(x, weight, output[1], output[2])
     ctx.bias_f32 = bias is not None and bias.dtype == torch.float32
     ctx.set_materialize_grads(False)
@@ -473,7 +474,8 @@ def _(dh, dlast, x, gate, states, lengths, dim, form, reverse):
 
 
 def _gated_scan_setup(ctx, inputs, output):
-    x, gate, _, lengths, ctx.dim, ctx.form, ctx.reverse = inputs
+    x, gate, h0, lengths, ctx.dim, ctx.form, ctx.reverse = inputs
+    ops_seq.refuse_held_leaves(x, gate, h0)
     ctx.save_for_backward(x, gate, output[2], lengths)
     ctx.set_materialize_grads(False)
 

@@ -132,7 +132,8 @@ class FusedAdamW:
     clip_grad_norm_(max_norm=grad_clip) folded in.
 
     state_bits = 8 keeps exp_avg and exp_avg_sq as 8-bit floats with a power-of-two scale for every 256 elements: 2 bytes a parameter
-    instead of 8; `seed` is their rounding's.  A parameter whose .grad is None is left alone in that step.
+    instead of 8; `seed` is their rounding's.  A parameter whose .grad is None is left alone in that step; the bias
+    corrections count the optimiser's steps, for all parameters alike.
     16-bit parameters that something else has written (a checkpoint, say) are taken over into the master copy by sync_master().
     capturable = True keeps step and lr on the device, so that a captured step counts on at every replay; `lr` is then taken over
     from param_groups by every step outside a capture, or by sync_lr()."""

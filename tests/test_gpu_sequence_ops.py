@@ -811,7 +811,7 @@ def test_refusals_without_the_native_calls(torch_mod, monkeypatch):
 def test_more_refusals(torch_mod):
     """lazily negated and sparse tensors, a state that is no buffer of its own, gradients through the step"""
     torch = torch_mod
-    from sound_bubble_amd import functional as F
+    from sound_bubble_amd import functional as F, ops
     from sound_bubble_amd._lib import SoundBubbleHipError as E
     neg = torch.randn(4, 8, dtype=torch.complex64, device="cuda").conj().imag
     assert neg.is_neg()
@@ -821,6 +821,45 @@ def test_more_refusals(torch_mod):
                  lambda: F.gated_scan_step(leaf, h, h), lambda: F.gated_scan_step(h, h, h.t().contiguous().t()), lambda: F.layer_norm([1.0])):
         with pytest.raises(E):
             call()
+    p = torch.ones(4, 8, device="cuda")
+    for g in (neg, h.to_sparse()):
+        with pytest.raises(E, match="gradient 0"):
+            ops.adamw_step([p], [g], ops.adamw_state([p]), 1, lr=0.1)
+    assert p.eq(1).all()
+
+
+@pytest.mark.parametrize("how", ["native", "python"])
+def test_lazily_negated_gradients(torch_mod, monkeypatch, how):
+    """a gradient that reaches the backward pass as a negated view"""
+    torch = torch_mod
+    from sound_bubble_amd import functional as F, ops_seq
+    monkeypatch.setattr(ops_seq, "_PYTHON", how == "python")
+    x = torch.randn(3, 40, 8, generator=gen(torch, 5), device="cuda", requires_grad=True)
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    dy = torch.randn(3, 40, 8, dtype=torch.complex64, device="cuda").conj().imag
+    assert dy.is_neg()
+    y, (h, last) = F.layer_norm(x, w), F.gated_scan(x, x * 2)
+    dl = dy[:, 0]
+    for lazy, plain in zip(torch.autograd.grad((y, h, last), (x, w), (dy, dy, dl), retain_graph=True),
+                           torch.autograd.grad((y, h, last), (x, w), (dy.resolve_neg(), dy.resolve_neg(), dl.resolve_neg()))):
+        assert torch.equal(lazy, plain)
+
+
+@pytest.mark.parametrize("how", ["native", "python"])
+def test_tangents_are_refused(torch_mod, monkeypatch, how):
+    """forward-mode differentiation has no rule here: said, not dropped"""
+    torch = torch_mod
+    from sound_bubble_amd import functional as F, ops_seq
+    import torch.autograd.forward_ad as fwAD
+    monkeypatch.setattr(ops_seq, "_PYTHON", how == "python")
+    x, t = torch.randn(2, 5, 8, device="cuda"), torch.ones(2, 5, 8, device="cuda")
+    with torch.enable_grad(), fwAD.dual_level():
+        d = fwAD.make_dual(x, t)
+        for call in (lambda: F.layer_norm(d), lambda: F.layer_norm(x, d[0, 0]), lambda: F.gated_scan(d, x), lambda: F.gated_scan(x, d),
+                     lambda: F.gated_scan_step(d, x, torch.zeros_like(x))):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+        assert torch.equal(F.layer_norm(x), F.layer_norm(x.clone()))
 
 
 def test_adamw_refuses_what_it_cannot_mean(torch_mod):
@@ -839,22 +878,29 @@ def test_adamw_refuses_what_it_cannot_mean(torch_mod):
     assert p.eq(1).all()
 
 
-def test_capture_refuses_leaves_of_a_live_eager_graph(torch_mod):
+@pytest.mark.parametrize("how", ["native", "python", "dispatcher"])
+def test_capture_refuses_leaves_of_a_live_eager_graph(torch_mod, monkeypatch, how):
     """the forward call under capture says so (its backward pass would end the process); without the eager graph it goes on"""
     torch = torch_mod
-    from sound_bubble_amd import functional as F
+    from sound_bubble_amd import functional as F, ops_seq
     from sound_bubble_amd._lib import SoundBubbleHipError as E
+    monkeypatch.setattr(ops_seq, "_PYTHON", how == "python")
+    norm, scan = F.layer_norm, F.gated_scan
+    if how == "dispatcher":
+        from sound_bubble_amd import torch_ops  # noqa: F401
+        norm = lambda x, w: torch.ops.sound_bubble.layer_norm(x, w, None, 1e-5)[0]  # noqa: E731
+        scan = lambda x, z: torch.ops.sound_bubble.gated_scan(x, z, None, None, 1, "sigmoid", False)  # noqa: E731
     x = torch.randn(4, 50, 16, device="cuda")
     w = torch.ones(16, device="cuda", requires_grad=True)
     z = torch.zeros(4, 50, 16, device="cuda", requires_grad=True)
-    eager = F.layer_norm(x, w), F.gated_scan(x, z)
+    eager = norm(x, w), scan(x, z)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
         graph = torch.cuda.CUDAGraph()
         graph.capture_begin()
         try:
-            for call in (lambda: F.layer_norm(x, w), lambda: F.gated_scan(x, z)):
+            for call in (lambda: norm(x, w), lambda: scan(x, z)):
                 with pytest.raises(E, match="eager graph"):
                     call()
             keep = x + 1
@@ -862,10 +908,10 @@ def test_capture_refuses_leaves_of_a_live_eager_graph(torch_mod):
             graph.capture_end()
     torch.cuda.current_stream().wait_stream(s)
     del eager, keep
-    want = torch.autograd.grad(F.layer_norm(x, w).sum() + F.gated_scan(x, z)[0].sum(), (w, z))
+    want = torch.autograd.grad(norm(x, w).sum() + scan(x, z)[0].sum(), (w, z))
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        got = torch.autograd.grad(F.layer_norm(x, w).sum() + F.gated_scan(x, z)[0].sum(), (w, z))
+        got = torch.autograd.grad(norm(x, w).sum() + scan(x, z)[0].sum(), (w, z))
     for _ in range(3):
         graph.replay()
         torch.cuda.synchronize()
