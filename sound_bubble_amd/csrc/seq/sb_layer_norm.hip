@@ -262,7 +262,8 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_bwd_kernel(sb_laye
   if (!a.scratch) return;
   float* out[2] = {a.scratch + (int64_t)blockIdx.x * a.n, a.scratch + ((int64_t)gridDim.x + blockIdx.x) * a.n};
 #pragma unroll
-  for (int which = 0; which < 2; ++which)
+  for (int which = 0; which < 2; ++which) {
+    if (which ? !a.db : !a.dw) continue;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       Vec<float, V> o;
@@ -280,6 +281,7 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_bwd_kernel(sb_laye
       }
       cols.store(out[which], o, k);
     }
+  }
 }
 
 // rows wider than a workgroup's registers: dx only, two passes over the row
