@@ -26,6 +26,7 @@ TORCH_SOURCE = os.path.join(CSRC, "seq", "sb_seq_torch.cpp")
 def torch_lib_cmd():
     """the compiler line of libsoundbubble_torch.so (torch is looked up, not imported)"""
     import importlib.util
+    import sysconfig
     spec = importlib.util.find_spec("torch")
     if spec is None:
         raise RuntimeError("libsoundbubble_torch.so needs an installed torch")
@@ -33,7 +34,7 @@ def torch_lib_cmd():
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-D_GLIBCXX_USE_CXX11_ABI=1",
             "-I" + os.path.join(t, "include"), "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(rocm, "include"),
-            TORCH_SOURCE, "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-lamdhip64", "-ltorch_cpu", "-ltorch"]
+            "-I" + sysconfig.get_paths()["include"], TORCH_SOURCE, "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-lamdhip64", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
 
 
 def csrc_digest():

@@ -5,11 +5,18 @@
 // These are the plain calls only.  Whatever is out of the ordinary -- a wrong type, nothing to compute, a copy that Python has to decide on --
 // is "not taken" (an empty list, 0): sound_bubble_amd/ops_seq.py then handles it, or says what is wrong.  The entry points' addresses come
 // from there too (bind), so that one library serves both.
+//
+// Layer norm and scan are operators of the dispatcher (0.7 us a call).  AdamW's lists of tensors are not: 160 parameters and gradients cost the
+// dispatcher 25 us, the module function below 2.
+#include <Python.h>
+
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
@@ -320,25 +327,33 @@ std::vector<Tensor> gated_scan_step(const Tensor& x, const Tensor& gate, const T
 }
 
 // ---- AdamW ----
-// 1: done, 0: not taken (nothing has been touched).  `state`: exp_avg, exp_avg_sq, their scales (8 bits), master (16-bit parameters)
-int64_t adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& state, int64_t bits, int64_t step,
-                   const Maybe& step_dev, double lr, const Maybe& lr_dev, double beta1, double beta2, double eps, double weight_decay, double gscale,
-                   double clip, int64_t seed, int64_t guard_word, int64_t skipped) {
+using Tensors = std::vector<const Tensor*>;      // (the caller's)
+struct AdamwCall {
+  Tensors params, grads, state;      // state: exp_avg, exp_avg_sq, their scales (8 bits), master (16-bit parameters)
+  int64_t bits, step;
+  Maybe step_dev, lr_dev;
+  double lr, beta1, beta2, eps, weight_decay, gscale, clip;
+  uint32_t seed;
+  const void* guard_word; void* skipped;
+};
+// 1: done, 0: not taken (nothing has been touched)
+int adamw_step(const AdamwCall& call) {
+  const auto& [params, grads, state, bits, step, step_dev, lr_dev, lr, beta1, beta2, eps, weight_decay, gscale, clip, seed, guard_word, skipped] = call;
   const size_t count = params.size();
-  if (count == 0 || count != grads.size() || !plain(params[0])) return 0;
-  const auto device = params[0].device();
-  const auto ptype = params[0].scalar_type(), gtype = grads[0].scalar_type();
+  if (count == 0 || count != grads.size() || !plain(*params[0])) return 0;
+  const auto device = params[0]->device();
+  const auto ptype = params[0]->scalar_type(), gtype = grads[0]->scalar_type();
   if (gtype != ptype && gtype != at::kFloat) return 0;
   int64_t blocks = 0;
   for (size_t i = 0; i < count; ++i) {      // (one pair of types, a gradient for each: the usual call)
-    const Tensor &p = params[i], &g = grads[i];
+    const Tensor &p = *params[i], &g = *grads[i];
     if (!plain(p) || !plain(g) || p.device() != device || g.device() != device || p.scalar_type() != ptype || g.scalar_type() != gtype ||
         p.sizes() != g.sizes() || p.numel() == 0 || !p.is_contiguous() || !g.is_contiguous())
       return 0;
     blocks += (p.numel() + SB_ADAMW_BLOCK - 1) / SB_ADAMW_BLOCK;
   }
   std::vector<const void*> places(count);
-  for (size_t i = 0; i < count; ++i) places[i] = params[i].data_ptr();
+  for (size_t i = 0; i < count; ++i) places[i] = params[i]->data_ptr();
   std::sort(places.begin(), places.end());
   if (std::adjacent_find(places.begin(), places.end()) != places.end()) return 0;
   const auto rate = [](double v) { return v >= 0 && v < 1; };
@@ -347,7 +362,7 @@ int64_t adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>&
   const size_t slots_per = SB_ADAMW_NORM_SLOTS / ((count + SB_ADAMW_MAX - 1) / SB_ADAMW_MAX);
   if ((bits != 8 && bits != 32) || state.size() != buffers || blocks >= (1LL << 31) || slots_per == 0 || !(clip >= 0)) return 0;
   for (size_t i = 0; i < buffers; ++i) {
-    const Tensor& t = state[i];
+    const Tensor& t = *state[i];
     const bool scale = bits == 8 && (i == 2 || i == 3);
     const auto want = i + 1 == buffers && ptype != at::kFloat ? at::kFloat : bits == 32 ? at::kFloat : scale ? at::kFloat8_e8m0fnu : i == 0 ? at::kFloat8_e4m3fn : at::kFloat8_e5m2;
     if (!t.defined() || t.device() != device || t.layout() != at::kStrided || t.scalar_type() != want || !t.is_contiguous() ||
@@ -358,26 +373,26 @@ int64_t adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>&
     return 0;
   if (given(lr_dev) && !(lr_dev->is_cuda() && lr_dev->device() == device && lr_dev->scalar_type() == at::kFloat && lr_dev->numel() == 1)) return 0;
   const c10::OptionalDeviceGuard guard(device);
-  for (const Tensor& p : params) p.unsafeGetTensorImpl()->bump_version();
+  for (const Tensor* p : params) p->unsafeGetTensorImpl()->bump_version();
   sb_adamw_args a = {};
-  a.ptype = type_of(params[0]); a.gtype = type_of(grads[0]); a.bits = (int)bits;
-  a.m = ptr(state[0]); a.v = ptr(state[1]);
+  a.ptype = type_of(*params[0]); a.gtype = type_of(*grads[0]); a.bits = (int)bits;
+  a.m = ptr(*state[0]); a.v = ptr(*state[1]);
   if (bits == 8) {
-    a.m_scale = ptr(state[2]);
-    a.v_scale = ptr(state[3]);
+    a.m_scale = ptr(*state[2]);
+    a.v_scale = ptr(*state[3]);
   }
-  if (ptype != at::kFloat) a.master = ptr<float>(state[buffers - 1]);
+  if (ptype != at::kFloat) a.master = ptr<float>(*state[buffers - 1]);
   a.lr = lr; a.beta1 = beta1; a.beta2 = beta2; a.eps = eps; a.weight_decay = weight_decay;
   a.lr_dev = given(lr_dev) ? ptr<float>(*lr_dev) : nullptr;
   a.step_dev = given(step_dev) ? ptr<int32_t>(*step_dev) : nullptr;
-  a.step = (int32_t)step; a.seed = (uint32_t)seed;
+  a.step = (int32_t)step; a.seed = seed;
   a.gscale = (float)gscale; a.clip = (float)clip;
   a.guard = (const int*)guard_word; a.skipped = (int*)skipped;
-  void* stream = stream_of(params[0]);
+  void* stream = stream_of(*params[0]);
   const int64_t chunk = entry.adamw_chunk();
   Tensor part;
   if (clip > 0) {
-    part = at::empty({SB_ADAMW_NORM_SLOTS}, params[0].options().dtype(at::kDouble));
+    part = at::empty({SB_ADAMW_NORM_SLOTS}, params[0]->options().dtype(at::kDouble));
     a.norm_part = (const double*)part.data_ptr();
     a.norm_slots = (int)(slots_per * ((count + SB_ADAMW_MAX - 1) / SB_ADAMW_MAX));
   }
@@ -387,8 +402,8 @@ int64_t adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>&
       const size_t n = std::min<size_t>(SB_ADAMW_MAX, count - i0);
       int64_t first = 0;
       for (size_t j = 0; j < n; ++j) {
-        const Tensor& p = params[i0 + j];
-        a.t[j] = {p.data_ptr(), grads[i0 + j].data_ptr(), p.numel(), (int32_t)block, (int32_t)first};
+        const Tensor& p = *params[i0 + j];
+        a.t[j] = {p.data_ptr(), grads[i0 + j]->data_ptr(), p.numel(), (int32_t)block, (int32_t)first};
         block += (p.numel() + SB_ADAMW_BLOCK - 1) / SB_ADAMW_BLOCK;
         first += (p.numel() + chunk - 1) / chunk;
       }
@@ -403,6 +418,51 @@ int64_t adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>&
   return 1;
 }
 
+struct WithoutGil {
+  PyThreadState* state = PyEval_SaveThread();
+  ~WithoutGil() { PyEval_RestoreThread(state); }
+};
+bool tensors_of(PyObject* list, Tensors& out) {
+  if (!PyList_Check(list)) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(list);
+  out.reserve(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* t = PyList_GET_ITEM(list, i);
+    if (!THPVariable_Check(t)) return false;
+    out.push_back(&THPVariable_Unpack(t));
+  }
+  return true;
+}
+// adamw_step(params, grads, state, bits, step, step_dev, lr, lr_dev, beta1, beta2, eps, weight_decay, gscale, clip, seed, guard, skipped) -> bool
+PyObject* py_adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 17, "adamw_step takes 17 arguments, got ", n);
+  AdamwCall c;
+  if (!tensors_of(args[0], c.params) || !tensors_of(args[1], c.grads) || !tensors_of(args[2], c.state)) Py_RETURN_FALSE;
+  const auto maybe = [](PyObject* o) { return THPVariable_Check(o) ? Maybe(THPVariable_Unpack(o)) : Maybe(); };
+  c.bits = PyLong_AsLongLong(args[3]);
+  c.step = PyLong_AsLongLong(args[4]);
+  c.step_dev = maybe(args[5]);
+  c.lr_dev = maybe(args[7]);
+  double* const to[] = {&c.lr, &c.beta1, &c.beta2, &c.eps, &c.weight_decay, &c.gscale, &c.clip};
+  const int from[] = {6, 8, 9, 10, 11, 12, 13};
+  for (int i = 0; i < 7; ++i) *to[i] = PyFloat_AsDouble(args[from[i]]);
+  c.seed = (uint32_t)PyLong_AsUnsignedLongLong(args[14]);
+  c.guard_word = PyLong_AsVoidPtr(args[15]);
+  c.skipped = PyLong_AsVoidPtr(args[16]);
+  if (PyErr_Occurred()) return nullptr;
+  int done;
+  {
+    const WithoutGil without;
+    done = adamw_step(c);
+  }
+  return PyBool_FromLong(done);
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef functions[] = {{"adamw_step", (PyCFunction)(void*)py_adamw_step, METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "libsoundbubble_torch", nullptr, -1, functions, nullptr, nullptr, nullptr, nullptr};
+
 }  // namespace
 
 TORCH_LIBRARY(sound_bubble_seq, m) {
@@ -411,6 +471,6 @@ TORCH_LIBRARY(sound_bubble_seq, m) {
   m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor[]", layer_norm);
   m.def("gated_scan(Tensor x, Tensor gate, Tensor? h0, Tensor? lengths, int dim, int form, bool reverse) -> Tensor[]", gated_scan);
   m.def("gated_scan_step(Tensor x, Tensor gate, Tensor(a!) state, int form) -> Tensor[]", gated_scan_step);
-  m.def("adamw_step(Tensor[] params, Tensor[] grads, Tensor[] state, int bits, int step, Tensor? step_dev, float lr, Tensor? lr_dev, float beta1, "
-        "float beta2, float eps, float weight_decay, float gscale, float clip, int seed, int guard, int skipped) -> int", adamw_step);
 }
+
+PyMODINIT_FUNC PyInit_libsoundbubble_torch() { return PyModule_Create(&module); }

@@ -6,6 +6,8 @@ stream of the tensors' own device; what a call needs besides its results is allo
 """
 import ctypes as C
 import functools
+import importlib.machinery
+import importlib.util
 import itertools
 import os
 
@@ -28,12 +30,15 @@ _NATIVE = None      # the operators of libsoundbubble_torch.so, False: there is 
 
 
 class _Native:
-    def __init__(self):
-        lib = L.load()
+    def __init__(self, path):
+        lib, name = L.load(), "libsoundbubble_torch"
+        spec = importlib.util.spec_from_file_location(name, path, loader=importlib.machinery.ExtensionFileLoader(name, path))
+        self.module = importlib.util.module_from_spec(spec)      # (registers the operators too)
+        spec.loader.exec_module(self.module)
         ops = torch.ops.sound_bubble_seq
         ops.bind([C.cast(getattr(lib, name), C.c_void_p).value for name in _ENTRIES])
         self.layer_norm, self.gated_scan = ops.layer_norm.default, ops.gated_scan.default
-        self.gated_scan_step, self.adamw_step = ops.gated_scan_step.default, ops.adamw_step.default
+        self.gated_scan_step, self.adamw_step = ops.gated_scan_step.default, self.module.adamw_step
         self.refuse_held_leaves = ops.refuse_held_leaves.default
 
 
@@ -48,8 +53,7 @@ def _library():
         path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsoundbubble_torch.so")
         _NATIVE = False
         if os.path.exists(path):
-            torch.ops.load_library(path)
-            _NATIVE = _Native()
+            _NATIVE = _Native(path)
     return _NATIVE
 
 
@@ -430,8 +434,8 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
             done = fast.adamw_step(params, grads, [state[k] for k in keys], bits, step, step_dev, lr, lr_dev, *betas, eps, weight_decay, gscale, clip,
                                    seed & 0xFFFFFFFF, guard.data_ptr() if guard is not None else 0,
                                    skipped.data_ptr() if guard is not None and skipped is not None else 0)
-        except (RuntimeError, TypeError, KeyError):      # (what it is, is said below)
-            done = 0
+        except (RuntimeError, TypeError, KeyError, OverflowError):      # (what it is, is said below)
+            done = False
         if done:
             return
     if len(params) != len(grads):
