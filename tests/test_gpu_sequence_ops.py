@@ -917,3 +917,51 @@ def test_capture_refuses_leaves_of_a_live_eager_graph(torch_mod, monkeypatch, ho
         torch.cuda.synchronize()
         F.layer_norm(x)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_more_than_2_31_elements(torch_mod):
+    """offsets that pass 32 bits: the far end of a large tensor is what the same rows, steps and blocks give by themselves"""
+    torch = torch_mod
+    from sound_bubble_amd import ops
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GiB of free GPU memory")
+    n, rows, tail = 1024, (1 << 21) + 3, 100
+    x, dy = (torch.randn(rows, n, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    w = torch.randn(n, device="cuda").bfloat16()
+    y, mean, rstd = ops.layer_norm_fwd(x, w, None)
+    assert torch.equal(y[-tail:], ops.layer_norm_fwd(x[-tail:], w, None)[0])
+    dx = ops.layer_norm_bwd(dy, x, w, mean, rstd, want_dw=False, want_db=False)[0]
+    assert torch.equal(dx[-tail:], ops.layer_norm_bwd(dy[-tail:], x[-tail:], w, mean[-tail:], rstd[-tail:], want_dw=False, want_db=False)[0])
+    del y, dx, mean, rstd
+    # gates of 0: h is x, and dgate_t is dh_t x_{t-1}
+    gate = torch.zeros_like(x)
+    h, last, states = ops.gated_scan_fwd(x, gate, dim=0, form="decay")
+    assert torch.equal(h, x) and torch.equal(last, x[-1].float())
+    del h
+    dx, dgate, _ = ops.gated_scan_bwd(dy, None, x, gate, states, dim=0, form="decay")
+    assert torch.equal(dx, dy)
+    assert torch.equal(dgate[-tail:], (dy[-tail:].float() * x[-tail - 1:-1].float()).bfloat16())
+    del dx, dgate, gate, states, x, dy
+    # a strided view over as much memory: 3 sequences, more than 2^32 bytes apart
+    far = (1 << 30) + 5
+    big = torch.empty(2 * far + 64 * 48, device="cuda")
+    x = big.as_strided((3, 64, 48), (far, 48, 1))
+    x.copy_(torch.randn(3, 64, 48, device="cuda"))
+    dense = x.contiguous()
+    assert torch.equal(ops.layer_norm_fwd(x, None, None)[0], ops.layer_norm_fwd(dense, None, None)[0])
+    for a, b in zip(ops.gated_scan_fwd(x, x), ops.gated_scan_fwd(dense, dense)):
+        assert torch.equal(a, b)
+    states = ops.gated_scan_fwd(x, x)[2]
+    for a, b in zip(ops.gated_scan_bwd(x, None, x, x, states), ops.gated_scan_bwd(dense, None, dense, dense, states)):
+        assert torch.equal(a, b)
+    del big, x
+    size, tail = (1 << 31) + 300, 44 + 5 * 256      # (the tail begins with a block)
+    p, g = torch.zeros(size, device="cuda"), torch.zeros(size, device="cuda")
+    p[-tail:], g[-tail:] = torch.randn(tail, device="cuda"), torch.randn(tail, device="cuda")
+    q, gq = p[-tail:].clone(), g[-tail:].clone()
+    sp, sq = ops.adamw_state([p]), ops.adamw_state([q])
+    for step in (1, 2):
+        ops.adamw_step([p], [g], sp, step, lr=0.1, clip=0.5)
+        ops.adamw_step([q], [gq], sq, step, lr=0.1, clip=0.5)
+    assert torch.equal(p[-tail:], q) and not p[:-tail].any()
+    assert all(torch.equal(sp[k][-sq[k].numel():], sq[k]) for k in sq)
