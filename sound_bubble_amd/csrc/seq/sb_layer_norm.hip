@@ -9,10 +9,6 @@
 
 namespace {
 
-template <class T> SB_DEVINL float wload(const void* w, int wtype, int64_t i) {
-  return wtype == SB_F32 ? ((const float*)w)[i] : (float)((const T*)w)[i];
-}
-
 // sum over the group; a group larger than a wave goes through LDS (two buffers in turn: one barrier a sum)
 template <int L> struct Group {
   float* lds;
@@ -91,9 +87,12 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_fwd_kernel(sb_laye
   constexpr bool kAhead = L < 1024 || K < 4;      // (the registers of a workgroup of 1024 do not hold another row)
   Vec<T, V> xv[K], next[K];
   if constexpr (kAhead) cols.load(next, (const T*)a.x + row * a.ldx);
-  Vec<W, V> w[K], b[K];
-  if (a.w) cols.load(w, (const W*)a.w);
-  if (a.b) cols.load(b, (const W*)a.b);
+  constexpr bool kLean = K == 8;      // (nor w and b, which the caches hold: fp32 3000 x 32768 218 -> 176 us)
+  Vec<W, V> w[kLean ? 1 : K], b[kLean ? 1 : K];
+  if constexpr (!kLean) {
+    if (a.w) cols.load(w, (const W*)a.w);
+    if (a.b) cols.load(b, (const W*)a.b);
+  }
   const float rn = 1.f / (float)a.n;
   for (; row < a.rows; row += step) {
     if constexpr (kAhead) {
@@ -127,12 +126,17 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_fwd_kernel(sb_laye
     T* y = (T*)a.y + row * a.n;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
+      constexpr bool kHeld = !kLean;
+      if constexpr (kLean) {
+        if (a.w) w[0] = vload<W, V>((const W*)a.w + cols.at(k));
+        if (a.b) b[0] = vload<W, V>((const W*)a.b + cols.at(k));
+      }
       Vec<T, V> o;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float v = ((float)xv[k].v[i] - mean) * rstd;
-        if (a.w) v *= (float)w[k].v[i];
-        if (a.b) v += (float)b[k].v[i];
+        if (a.w) v *= (float)w[kHeld ? k : 0].v[i];
+        if (a.b) v += (float)b[kHeld ? k : 0].v[i];
         o.v[i] = (T)v;
       }
       cols.store(y, o, k);
@@ -145,7 +149,7 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_fwd_kernel(sb_laye
 }
 
 // rows wider than a workgroup's registers: three passes over the row, which the caches hold
-template <class T>
+template <class T, class W>
 __global__ __launch_bounds__(1024) void layer_norm_fwd_wide_kernel(sb_layer_norm_args a) {
   constexpr int V = vec_of<T>(), L = 1024;
   __shared__ float lds[2 * (L / 64)];
@@ -175,11 +179,15 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_wide_kernel(sb_layer_norm
     for (int64_t c = (int64_t)threadIdx.x * V; c < a.n; c += (int64_t)L * V) {
       const int m = (int)min((int64_t)V, a.n - c);
       Vec<T, V> v = vload_n<T, V>(x + c, m);
+      Vec<W, V> w, b;
+      if (a.w) w = vload_n<W, V>((const W*)a.w + c, m);
+      if (a.b) b = vload_n<W, V>((const W*)a.b + c, m);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float w = a.w && i < m ? wload<T>(a.w, a.wtype, c + i) : 1.f;
-        const float b = a.b && i < m ? wload<T>(a.b, a.wtype, c + i) : 0.f;
-        v.v[i] = (T)(((float)v.v[i] - mean) * rstd * w + b);
+        float r = ((float)v.v[i] - mean) * rstd;
+        if (a.w) r *= (float)w.v[i];
+        if (a.b) r += (float)b.v[i];
+        v.v[i] = (T)r;
       }
       vstore_n<T, V>(y + c, v, m);
     }
@@ -189,6 +197,10 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_wide_kernel(sb_layer_norm
     }
   }
 }
+
+// Whether a group's registers hold the sums of dw and db beside the rows; where not, a kernel of its own reads x and dy once more for them
+// (bf16 16384 x 16384: 512 us, with the sums inside and spilled 705; fp32 3000 x 24000: 296, the wide kernel's two passes 365)
+constexpr bool sums_inside(int L, int K, bool f32) { return L < 1024 || (f32 && K <= 4); }
 
 // dx of every row, and (scratch given) a row of partial sums of dw and db a workgroup: scratch[(0 | 1)][workgroup][n]
 template <class T, class W, int V, int L, int K>
@@ -201,6 +213,7 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_bwd_kernel(sb_laye
   const int64_t step = (int64_t)gridDim.x * G;
   int64_t row = (int64_t)blockIdx.x * G + threadIdx.x / L;
   constexpr bool kAhead = L < 1024 || K < 3;      // another row's loads ahead, where the registers hold it
+  constexpr bool kSums = sums_inside(L, K, V == 4);
   Vec<T, V> xv[K], gv[K], nx[K], ng[K];
   float mean, rstd, nmean = 0.f, nrstd = 0.f;
   const auto load = [&](int64_t r) __attribute__((always_inline)) {
@@ -212,11 +225,13 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_bwd_kernel(sb_laye
   if (kAhead && row < a.rows) load(row);
   Vec<W, V> w[K];
   if (a.w) cols.load(w, (const W*)a.w);
-  float dw[K][V], db[K][V];
+  float dw[kSums ? K : 1][V], db[kSums ? K : 1][V];
+  if constexpr (kSums) {
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
+      for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
+  }
   const float rn = 1.f / (float)a.n;
   for (; row < a.rows; row += step) {
     if constexpr (!kAhead) load(row);
@@ -238,8 +253,10 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_bwd_kernel(sb_laye
           const float q = a.w ? g * (float)w[k].v[i] : g;
           s1 += q;
           s2 += q * xh;
-          dw[k][i] += g * xh;
-          db[k][i] += g;
+          if constexpr (kSums) {
+            dw[k][i] += g * xh;
+            db[k][i] += g;
+          }
         }
     };
     if (cols.exact()) sums(std::true_type()); else sums(std::false_type());
@@ -259,6 +276,7 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_bwd_kernel(sb_laye
       cols.store(dx, o, k);
     }
   }
+  if constexpr (!kSums) return;
   if (!a.scratch) return;
   float* out[2] = {a.scratch + (int64_t)blockIdx.x * a.n, a.scratch + ((int64_t)gridDim.x + blockIdx.x) * a.n};
 #pragma unroll
@@ -268,7 +286,7 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_bwd_kernel(sb_laye
     for (int k = 0; k < K; ++k) {
       Vec<float, V> o;
 #pragma unroll
-      for (int i = 0; i < V; ++i) o.v[i] = which ? db[k][i] : dw[k][i];
+      for (int i = 0; i < V; ++i) o.v[i] = which ? db[kSums ? k : 0][i] : dw[kSums ? k : 0][i];
       if constexpr (G > 1) {      // the groups' sum, by the first group
         __syncthreads();
 #pragma unroll
@@ -285,7 +303,7 @@ __global__ __launch_bounds__(threads_of<L>()) void layer_norm_bwd_kernel(sb_laye
 }
 
 // rows wider than a workgroup's registers: dx only, two passes over the row
-template <class T>
+template <class T, class W>
 __global__ __launch_bounds__(1024) void layer_norm_bwd_wide_kernel(sb_layer_norm_bwd_args a) {
   constexpr int V = vec_of<T>(), L = 1024;
   __shared__ float lds[4 * (L / 64)];
@@ -300,9 +318,11 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_wide_kernel(sb_layer_norm
     for (int64_t c = (int64_t)threadIdx.x * V; c < a.n; c += (int64_t)L * V) {
       const int m = (int)min((int64_t)V, a.n - c);
       const Vec<T, V> xv = vload_n<T, V>(x + c, m), gv = vload_n<T, V>(dy + c, m);
+      Vec<W, V> w;
+      if (a.w) w = vload_n<W, V>((const W*)a.w + c, m);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float q = (float)gv.v[i] * (a.w && i < m ? wload<T>(a.w, a.wtype, c + i) : 1.f);
+        const float q = a.w ? (float)gv.v[i] * (float)w.v[i] : (float)gv.v[i];
         s1 += q;
         s2 += q * (((float)xv.v[i] - mean) * rstd);
       }
@@ -313,10 +333,12 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_wide_kernel(sb_layer_norm
     for (int64_t c = (int64_t)threadIdx.x * V; c < a.n; c += (int64_t)L * V) {
       const int m = (int)min((int64_t)V, a.n - c);
       const Vec<T, V> xv = vload_n<T, V>(x + c, m), gv = vload_n<T, V>(dy + c, m);
+      Vec<W, V> w;
+      if (a.w) w = vload_n<W, V>((const W*)a.w + c, m);
       Vec<T, V> o;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float q = (float)gv.v[i] * (a.w && i < m ? wload<T>(a.w, a.wtype, c + i) : 1.f);
+        const float q = a.w ? (float)gv.v[i] * (float)w.v[i] : (float)gv.v[i];
         o.v[i] = (T)(rstd * (q - s1 - ((float)xv.v[i] - mean) * rstd * s2));
       }
       vstore_n<T, V>(dx + c, o, m);
@@ -375,14 +397,16 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* sc
 
 // The groups in use.  Measured, us: forward, bf16 16384 x 4096: a wave with 8 vectors a lane 71, a workgroup of 256 with 2 47; backward, bf16
 // 16384 x 2048: a wave with 4 50, a workgroup with 1 44.  The backward pass's K vectors of x, dy, w, two of sums and the next row's have to
-// fit the registers: 128 a lane in a workgroup of 1024, 256 in one of 512 (fp16 2309 x 16384: 512 x 4 158, 1024 x 2 123).
+// fit the registers: 128 a lane in a workgroup of 1024, 256 in one of 512 (fp16 2309 x 16384: 512 x 4 158, 1024 x 2 without the sums 81; fp16
+// 3000 x 32768: 1024 x 4 317, the wide kernel 254; forward, fp16 3000 x 50000: 1024 x 8 590, the wide kernel 213).
 constexpr bool taken(int L, int K, bool f32, bool backward) {
   if (L <= 64) return K <= (backward ? 2 : 4);
-  if (!backward) return !(L == 1024 && K == 2);
-  return f32 ? (K <= 4 && !(L == 512 && K == 4)) : (L == 1024 ? K == 2 : L == 512 ? K == 3 : true);
+  if (!backward) return !(L == 1024 && (K == 2 || (!f32 && K > 4)));
+  return f32 ? !(L == 512 && K == 4) : (L == 1024 ? K <= 3 : L == 512 ? K == 3 : true);
 }
-// workgroups of the forward pass, which walk over the rows: 1.45 M x 32 fp32: 68 us, with 2048 77; fp16 2309 x 16384: 36, with 2048 45
-constexpr int64_t kFwdGrid = 1024;
+// waves of the forward pass, whose groups walk over the rows: 1.45 M x 32 fp32: 68 us, with 8192 waves 77, with 2048 84; fp16 2309 x 16384:
+// 31, with 8192 36
+constexpr int64_t kFwdWaves = 4096;
 // elements of a vector: 16 bytes, or one where the row is shorter than that
 int vec_for(int64_t n, int xtype) {
   const int vec = xtype == SB_F32 ? 4 : 8;
@@ -436,7 +460,7 @@ template <class F> int with_types(int xtype, int wtype, F&& f) {
 // rows one a compute unit (fp16 2309 x 10007: 256 54 us, 512 77 us), with many two (bf16 16384 x 2048: 512 44 us, 256 50 us)
 int64_t bwd_grid(int64_t rows, int64_t n, int xtype) {
   const Shape s = shape_of(n, xtype, true);
-  if (!s.L) return std::min<int64_t>(rows, 128);
+  if (!s.L || !sums_inside(s.L, s.K, xtype == SB_F32)) return std::min<int64_t>(rows, 128);      // (of the kernel for the sums alone)
   const int64_t per = s.L >= 256 ? 1 : 256 / s.L;
   return std::min<int64_t>((rows + per - 1) / per, s.L >= 256 && rows < 8192 ? 256 : 512);
 }
@@ -454,11 +478,11 @@ extern "C" int sb_layer_norm_fwd(const sb_layer_norm_args* ap, void* stream) {
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(wt)>;
     if (!s.L) {
-      hipLaunchKernelGGL((layer_norm_fwd_wide_kernel<T>), dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(1024), 0, (hipStream_t)stream, a);
+      hipLaunchKernelGGL((layer_norm_fwd_wide_kernel<T, W>), dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(1024), 0, (hipStream_t)stream, a);
     } else {
       const int rc = with_shape<T, false>(a.n, s, [&](auto V, auto L, auto K) -> int {
         constexpr int per = threads_of<L.value>() / L.value;
-        const int64_t grid = std::min<int64_t>((a.rows + per - 1) / per, kFwdGrid);
+        const int64_t grid = std::min<int64_t>((a.rows + per - 1) / per, kFwdWaves * 64 / threads_of<L.value>());
         hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, V.value, L.value, K.value>), dim3((unsigned)grid), dim3(threads_of<L.value>()), 0, (hipStream_t)stream, a);
         return 0;
       });
@@ -482,19 +506,23 @@ extern "C" int sb_layer_norm_bwd(const sb_layer_norm_bwd_args* ap, void* stream)
   return with_types(a.xtype, a.wtype, [&](auto* t, auto* wt) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(wt)>;
+    const bool apart = a.rows > 0 && (!s.L || !sums_inside(s.L, s.K, std::is_same_v<T, float>));
     if (a.rows > 0 && !s.L) {
-      hipLaunchKernelGGL((layer_norm_bwd_wide_kernel<T>), dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(1024), 0, (hipStream_t)stream, a);
-      SB_CHECK_LAUNCH();
-      if (sums) hipLaunchKernelGGL((layer_norm_cols_kernel<T>), dim3((unsigned)((a.n / vec_of<T>() + 256) / 256), grid), dim3(256), 0, (hipStream_t)stream, a, grid);
+      hipLaunchKernelGGL((layer_norm_bwd_wide_kernel<T, W>), dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(1024), 0, (hipStream_t)stream, a);
     } else if (a.rows > 0) {
       if (!sums) a.scratch = nullptr;
       const int rc = with_shape<T, true>(a.n, s, [&](auto V, auto L, auto K) -> int {
-        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, V.value, L.value, K.value>), dim3(grid), dim3(threads_of<L.value>()), 0, (hipStream_t)stream, a);
+        const int wgs = apart ? (int)std::min<int64_t>(a.rows, 512) : grid;
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, V.value, L.value, K.value>), dim3(wgs), dim3(threads_of<L.value>()), 0, (hipStream_t)stream, a);
         return 0;
       });
       if (rc) return rc;
     }
     SB_CHECK_LAUNCH();
+    if (apart && sums) {
+      hipLaunchKernelGGL((layer_norm_cols_kernel<T>), dim3((unsigned)((a.n / vec_of<T>() + 256) / 256), grid), dim3(256), 0, (hipStream_t)stream, a, grid);
+      SB_CHECK_LAUNCH();
+    }
     if (sums) {      // (no rows: no partial sums either, the sums are 0)
       hipLaunchKernelGGL((layer_norm_reduce_kernel<W>), dim3((unsigned)((a.n + 31) / 32), 2), dim3(1024), 0, (hipStream_t)stream, a.scratch,
                          a.rows > 0 ? grid : 0, a.n, a.dw, a.db);
