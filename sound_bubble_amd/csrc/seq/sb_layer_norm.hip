@@ -396,11 +396,12 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* sc
 }
 
 // The groups in use.  Measured, us: forward, bf16 16384 x 4096: a wave with 8 vectors a lane 71, a workgroup of 256 with 2 47; backward, bf16
-// 16384 x 2048: a wave with 4 50, a workgroup with 1 44.  The backward pass's K vectors of x, dy, w, two of sums and the next row's have to
-// fit the registers: 128 a lane in a workgroup of 1024, 256 in one of 512 (fp16 2309 x 16384: 512 x 4 158, 1024 x 2 without the sums 81; fp16
-// 3000 x 32768: 1024 x 4 317, the wide kernel 254; forward, fp16 3000 x 50000: 1024 x 8 590, the wide kernel 213).
+// 16384 x 2048: a wave with 4 50, a workgroup with 1 44, 50000 x 1280: a wave with 3 89, a workgroup with 1 115.  The backward pass's K vectors
+// of x, dy, w, two of sums and the next row's have to fit the registers: 128 a lane in a workgroup of 1024, 256 in one of 512 (fp16 2309 x
+// 16384: 512 x 4 158, 1024 x 2 without the sums 81; fp16 3000 x 32768: 1024 x 4 317, the wide kernel 254; forward, fp16 3000 x 50000:
+// 1024 x 8 590, the wide kernel 213).
 constexpr bool taken(int L, int K, bool f32, bool backward) {
-  if (L <= 64) return K <= (backward ? 2 : 4);
+  if (L <= 64) return K <= (backward ? 3 : 4);
   if (!backward) return !(L == 1024 && (K == 2 || (!f32 && K > 4)));
   return f32 ? !(L == 512 && K == 4) : (L == 1024 ? K <= 3 : L == 512 ? K == 3 : true);
 }
@@ -422,7 +423,8 @@ Shape shape_of(int64_t n, int xtype, bool backward) {
     while (L < vecs) L *= 2;
     return {L, 1};
   }
-  for (const Shape s : {Shape{64, 2}, {64, 4}, {256, 1}, {256, 2}, {256, 3}, {256, 4}, {512, 3}, {512, 4}, {1024, 2}, {1024, 3}, {1024, 4}, {1024, 6}, {1024, 8}})
+  for (const Shape s : {Shape{64, 2}, {64, 3}, {64, 4}, {256, 1}, {256, 2}, {256, 3}, {256, 4}, {512, 3}, {512, 4}, {1024, 2}, {1024, 3}, {1024, 4},
+                        {1024, 6}, {1024, 8}})
     if ((int64_t)s.L * s.K >= vecs && taken(s.L, s.K, xtype == SB_F32, backward)) return s;
   return {0, 0};
 }
@@ -441,7 +443,7 @@ template <class T, bool BACKWARD, class F> int with_shape(int64_t n, Shape s, F&
 #define SB_CASE(l, k) \
   if constexpr (taken(l, k, std::is_same_v<T, float>, BACKWARD)) \
     if (s.L == l && s.K == k) return f(vec, std::integral_constant<int, l>(), std::integral_constant<int, k>());
-  SB_CASE(1, 1) SB_CASE(2, 1) SB_CASE(4, 1) SB_CASE(8, 1) SB_CASE(16, 1) SB_CASE(32, 1) SB_CASE(64, 1) SB_CASE(64, 2) SB_CASE(64, 4)
+  SB_CASE(1, 1) SB_CASE(2, 1) SB_CASE(4, 1) SB_CASE(8, 1) SB_CASE(16, 1) SB_CASE(32, 1) SB_CASE(64, 1) SB_CASE(64, 2) SB_CASE(64, 3) SB_CASE(64, 4)
   SB_CASE(256, 1) SB_CASE(256, 2) SB_CASE(256, 3) SB_CASE(256, 4) SB_CASE(512, 3) SB_CASE(512, 4)
   SB_CASE(1024, 2) SB_CASE(1024, 3) SB_CASE(1024, 4) SB_CASE(1024, 6) SB_CASE(1024, 8)
 #undef SB_CASE

@@ -68,7 +68,7 @@ def norm_reference(torch, x, w, b, eps, dy=None):
     return y, e_y, dx, e_dx, dw, e_dw, db, e_db
 
 
-NORM_SHAPES = [(1, 1), (5, 1), (3, 7), (145, 32), (1000, 33), (64, 64), (17, 255), (4, 256), (9, 257), (33, 1000), (7, 1024), (5, 1025), (6, 2049),
+NORM_SHAPES = [(1, 1), (5, 1), (3, 7), (145, 32), (1000, 33), (64, 64), (17, 255), (4, 256), (9, 257), (9, 600), (33, 1000), (7, 1024), (5, 1025), (6, 2049),
                (700, 4096), (3, 10007), (5, 13001), (9, 16384), (2, 16385), (4, 20005), (3, 24570), (2, 30001), (3, 32768), (2, 40001), (3, 70001)]
 
 
