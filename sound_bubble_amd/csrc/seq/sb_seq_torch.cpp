@@ -6,8 +6,8 @@
 // is "not taken" (an empty list, 0): sound_bubble_amd/ops_seq.py then handles it, or says what is wrong.  The entry points' addresses come
 // from there too (bind), so that one library serves both.
 //
-// Layer norm and scan are operators of the dispatcher (0.7 us a call).  AdamW's lists of tensors are not: 160 parameters and gradients cost the
-// dispatcher 25 us, the module function below 2.
+// Layer norm and scan are operators of the dispatcher (0.7 us a call).  AdamW's lists of tensors are not: a step over 160 parameters is 39 us of
+// host time by the dispatcher, 18 by the module's function.
 #include <Python.h>
 
 #include <ATen/ATen.h>
