@@ -41,7 +41,7 @@ int64_t sb_layer_norm_bwd_scratch(int64_t rows, int64_t n, int xtype);
 int sb_layer_norm_bwd(const sb_layer_norm_bwd_args* a, void* stream);
 
 /* ---- gated linear recurrence over the middle axis of [outer, steps, inner] ----
- *   form SB_SCAN_DECAY:    h_t = g_t h_{t-1} + x_t
+ *   form SB_SCAN_DECAY:    h_t = g_t h_{t-1} + x_t       (products of 16 gates in a row have to stay within float32)
  *   form SB_SCAN_SIGMOID:  h_t = s(g_t) h_{t-1} + (1 - s(g_t)) x_t,  s the logistic function
  * x of type xtype, gate of type gtype (xtype or SB_F32); h has x's type; h0 (nullable: zeros), h_last fp32 [outer, inner].
  * x / gate / dh: outer stride so_*, step stride st_*, inner axis dense.  h, dx, dgate dense.

@@ -24,7 +24,8 @@ constexpr int S = 16, kMaxWaves = 8;
 // gate twice.  fp16 6 x 3001 x 1000 (752 waves) forward / backward, us: cut 68 / 94, whole 94 / 134.
 // A segment joins the pairs of all in front of it, 0.1 us each, and walks its own chunks, 2.4 us each in both kernels: of c chunks about
 // 5 sqrt(c) segments.  fp32 1 x 262144 x 16 forward / backward, us: 64 segments 217 / 258, 226 87 / 106; 1 x 65536 x 64: 64 49 / 56, 113 40 / 45.
-constexpr int kFewWaves = 1024, kWaves = 4096, kMaxSplits = 512;
+// (409 segments: the pairs and powers of as many as 512 pairs alone take.)
+constexpr int kFewWaves = 1024, kWaves = 4096, kMaxSplits = 409;
 
 struct Lay {
   int nw, splits;                  // waves along time, segments of time
@@ -176,6 +177,20 @@ template <class E> SB_DEVINL void kill_dead(E (&v)[S], unsigned live) {
   for (int s = 0; s < S; ++s) v[s] = live >> s & 1 ? v[s] : (E)0.f;
 }
 
+// The product of a segment's gates leaves float32 where they are beyond 1 ("decay": 256 gates of 1.5 are 2^150), and an infinite product times
+// a state of 0 is NaN where the recurrence stays 0.  It is kept as A 2^power, 0.5 <= |A| < 1 (or 0, infinite, NaN, power whatever), which
+// rounds as the product itself does; the power is taken out every S gates, so that only products of S have to stay within float32.
+SB_DEVINL void take_power(float& A, int& power) {
+  constexpr int kMost = 1 << 24;      // (of a sum: nothing comes back from there within a segment)
+  power = min(max(power + __builtin_amdgcn_frexp_expf(A), -kMost), kMost);
+  A = __builtin_amdgcn_frexp_mantf(A);
+}
+// A 2^power c + B; one rounding where A 2^power is a normal number
+SB_DEVINL float join_power(float A, int power, float c, float B) {
+  if (power >= -125 && power <= 128) return __builtin_fmaf(__builtin_ldexpf(A, power), c, B);
+  return __builtin_ldexpf(A * c, power) + B;
+}
+
 // the pairs of a workgroup's waves, two buffers in turn: [turn][wave][lane]
 struct Pairs {
   float2* lds;
@@ -197,8 +212,13 @@ struct Pairs {
   }
 };
 
+// k.agg: the segments' pairs [split][A | B][plane], then ("decay") the products' powers [split][plane] in 16 bits: behind +-1000 any
+// state but 0 is infinite, any finite one 0
+SB_DEVINL int16_t* powers_of(const Kargs& k) { return (int16_t*)(k.agg + 2 * k.splits * k.outer * k.inner); }
+int64_t pairs_floats(int64_t splits, int64_t plane) { return 2 * (splits + (splits + 3) / 4) * plane; }
+
 // state in front of segment `split`: h0 and the pairs of the earlier ones (UP), dlast and those of the later ones (!UP)
-template <bool UP> SB_DEVINL float fold_splits(const float* start, const Place& p, const Kargs& k, int split) {
+template <int FORM, bool UP> SB_DEVINL float fold_splits(const float* start, const Place& p, const Kargs& k, int split) {
   const int64_t plane = k.outer * k.inner;
   if (!p.on) return 0.f;
   float carry = start ? start[p.q] : 0.f;
@@ -206,15 +226,17 @@ template <bool UP> SB_DEVINL float fold_splits(const float* start, const Place& 
   constexpr int N = 16;
   for (int j0 = 0; j0 < n; j0 += N) {      // (the loads of N pairs at once: one after the other they cost a trip to memory each)
     float A[N], B[N];
+    int power[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int j = UP ? j0 + i : k.splits - 1 - j0 - i;
+      power[i] = FORM == SB_SCAN_DECAY && j0 + i < n ? powers_of(k)[j * plane + p.q] : 0;
       A[i] = j0 + i < n ? k.agg[(2 * j) * plane + p.q] : 1.f;
       B[i] = j0 + i < n ? k.agg[(2 * j + 1) * plane + p.q] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (j0 + i < n) carry = __builtin_fmaf(A[i], carry, B[i]);
+      if (j0 + i < n) carry = FORM == SB_SCAN_DECAY ? join_power(A[i], power[i], carry, B[i]) : __builtin_fmaf(A[i], carry, B[i]);
   }
   return carry;
 }
@@ -232,6 +254,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_pair_kernel(Kargs k
   const void* from = UP ? k.x : k.dh;
   const int64_t so = UP ? k.so_x : k.so_d, st = UP ? k.st_x : k.st_d, step = UP ? S : -S;
   float carry = 0.f, whole = 1.f;
+  int power = 0;
   T x[S];
   G g[S];
 #pragma unroll
@@ -262,6 +285,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_pair_kernel(Kargs k
       whole *= a[s];
       carry = UP ? __builtin_fmaf(a[s], carry, ol[s] * xf[s]) : a[s] * (xf[s] + carry);
     }
+    if constexpr (FORM == SB_SCAN_DECAY) take_power(whole, power);
   };
   int64_t t = UP ? first : last;
   int64_t left = (last - first) / S + 1;
@@ -274,16 +298,30 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_pair_kernel(Kargs k
   }
   if (p.waves > 1) {
     pairs.at(0, p.wave) = make_float2(whole, carry);
+    if constexpr (FORM == SB_SCAN_DECAY) pairs.at(1, p.wave).x = __int_as_float(power);
     block_sync();
-    float in;
     carry = 0.f;
-    pairs.template join<UP>(0, -1, carry, in);
+    if constexpr (FORM == SB_SCAN_DECAY) {
+      power = 0;
+      for (int w = 0; w < p.waves; ++w) {
+        const int j = UP ? w : p.waves - 1 - w;
+        const float2 r = pairs.at(0, j);
+        const int q = __float_as_int(pairs.at(1, j).x);
+        carry = join_power(r.x, q, carry, r.y);
+        power += q;
+      }
+    } else {
+      float in;
+      pairs.template join<UP>(0, -1, carry, in);
+    }
     whole = pairs.product(0);
+    if constexpr (FORM == SB_SCAN_DECAY) take_power(whole, power);
   }
   if (p.wave == 0 && p.on) {
     const int64_t plane = k.outer * k.inner;
     k.agg[(2 * split) * plane + p.q] = whole;
     k.agg[(2 * split + 1) * plane + p.q] = carry;
+    if constexpr (FORM == SB_SCAN_DECAY) powers_of(k)[split * plane + p.q] = (int16_t)min(max(power, -1000), 1000);
   }
 }
 
@@ -295,7 +333,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(Kargs k)
   const Pairs pairs{lds, p.waves};
   const int split = blockIdx.y;
   const int64_t c0 = k.chunks * split / k.splits, c1 = k.chunks * (split + 1) / k.splits, plane = k.outer * k.inner;
-  float carry = fold_splits<true>(k.h0, p, k, split);
+  float carry = fold_splits<FORM, true>(k.h0, p, k, split);
   T x[S];
   G g[S];
   const auto load = [&](int64_t t, bool full) __attribute__((always_inline)) {
@@ -364,7 +402,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(Kargs k)
   const Pairs down{lds, p.waves}, up{lds + 2 * 64 * p.waves, p.waves};
   const int split = blockIdx.y;
   const int64_t c0 = k.chunks * split / k.splits, c1 = k.chunks * (split + 1) / k.splits, plane = k.outer * k.inner;
-  float carry = fold_splits<false>(k.dlast, p, k, split);
+  float carry = fold_splits<FORM, false>(k.dlast, p, k, split);
   T x[S], d[S];
   G g[S];
   float state = 0.f;
@@ -512,7 +550,7 @@ extern "C" int sb_gated_scan_plan(int64_t outer, int64_t steps, int64_t inner, i
   if (outer == 0 || steps == 0 || inner == 0) return 0;
   const Lay l = lay_of(outer, steps, inner);
   *chunks = l.chunks;
-  *fwd_scratch = *bwd_scratch = l.splits > 1 ? 2 * l.splits * outer * inner : 0;
+  *fwd_scratch = *bwd_scratch = l.splits > 1 ? pairs_floats(l.splits, outer * inner) : 0;
   return 0;
 }
 

@@ -91,8 +91,8 @@ class GatedScanFn(torch.autograd.Function):
 def gated_scan(x, gate, h0=None, *, dim=1, form="sigmoid", reverse=False, lengths=None):
     """-> (h, last): h_t = a_t h_{t-1} + b_t along axis `dim`; last (float32) is the state behind the last step.
 
-    form "sigmoid": a = sigmoid(gate), b = (1 - a) x; "decay": a = gate, b = x.  A chunk of up to 256 steps is joined by products of its
-    gates: with "decay" gates beyond 1 in magnitude, those products have to stay within float32.
+    form "sigmoid": a = sigmoid(gate), b = (1 - a) x; "decay": a = gate, b = x.  Steps are joined by products of gates: with "decay"
+    gates beyond 1 in magnitude, products of 16 of them in a row have to stay within float32 (longer ones need not).
     h0: float32, x's shape without `dim` (None: zeros).  reverse: from the last step to the first.
     lengths (int64 / int32, x.shape[:dim]): a padded batch; steps at and behind a sequence's length leave its state alone, their
     outputs and gradients are 0 and their inputs are not looked at (reverse: the walk begins at a sequence's last own step).

@@ -1,0 +1,79 @@
+"""Sequence-block operators at the edges of their arguments, on the GPU, against their definitions in 64 bits."""
+import pytest
+
+from test_gpu_sequence_ops import U, gen, near
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- gated scan: gates beyond 1 ----
+def walk(torch, x, gate, h0, dh, dlast, reverse):
+    """the "decay" recurrence along axis 1 in 64 bits: h, last, dx, dgate, dh0"""
+    x, gate, dh = (t.double().flip(1) if reverse else t.double() for t in (x, gate, dh))
+    T = x.shape[1]
+    h = torch.zeros_like(x[:, 0]) if h0 is None else h0.double()
+    before, hs, G = [], [], [None] * T
+    for t in range(T):
+        before.append(h)
+        h = gate[:, t] * h + x[:, t]
+        hs.append(h)
+    c = dlast.double()
+    for t in reversed(range(T)):
+        G[t] = dh[:, t] + c
+        c = gate[:, t] * G[t]
+    hs, before, G = (torch.stack(v, 1) for v in (hs, before, G))
+    out = {"h": hs, "dx": G, "dgate": G * before}
+    out = {k: v.flip(1) if reverse else v for k, v in out.items()}
+    return {**out, "last": h, "dh0": c}
+
+
+def check_walk(torch, x, gate, h0, dh, dlast, reverse):
+    """Every term is positive, so every result is off by the roundings of its terms' factors: a term is a product of at most T gates, T - 1
+    roundings however they are grouped, and as many additions at most; 64 for the joins.  dgate has two such factors."""
+    from sound_bubble_amd import functional as F, ops_seq
+    B, T, C = x.shape
+    assert ops_seq._scan_plan(B, T, C, ops_seq._TYPES[x.dtype])[1] > 0, "time is cut at this size"
+    leaves = [t.detach().requires_grad_(True) for t in (x, gate, h0) if t is not None]
+    h, last = F.gated_scan(leaves[0], leaves[1], leaves[2] if h0 is not None else None, form="decay", reverse=reverse)
+    grads = torch.autograd.grad((h, last), leaves, (dh, dlast))
+    got = {"h": h.detach(), "last": last.detach(), **dict(zip(("dx", "dgate", "dh0"), grads))}
+    want = walk(torch, x, gate, h0, dh, dlast, reverse)
+    for k, v in got.items():
+        assert want[k].abs().max() < 1e37
+        near(torch, v, want[k], (2 * T + 64) * U * (2 if k == "dgate" else 1) * want[k] + 2.0 ** -140, k)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("top", [1.5, 200.0])
+@pytest.mark.parametrize("xt", ["float32", "bfloat16"])
+def test_gates_beyond_one_and_a_silent_start(torch_mod, xt, top, reverse):
+    """nothing but zeros until the last steps, a loss on the first ones only: everything between is 0, whatever the gates' products are"""
+    torch = torch_mod
+    xt, live = getattr(torch, xt), 10
+    g = gen(torch, 1)
+    r = lambda *s: torch.rand(*s, generator=g, device="cuda") + 0.25  # noqa: E731
+    x, dh = torch.zeros(2, 2048, 24, device="cuda", dtype=xt), torch.zeros(2, 2048, 24, device="cuda", dtype=xt)
+    gate = top * (1 - 0.1 * torch.rand(2, 2048, 24, generator=g, device="cuda"))
+    x[:, -live:], dh[:, :live] = r(2, live, 24).to(xt), r(2, live, 24).to(xt)
+    if reverse:
+        x, dh = x.flip(1).contiguous(), dh.flip(1).contiguous()
+    check_walk(torch, x, gate, None, dh, torch.zeros(2, 24, device="cuda"), reverse)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("shape", [(2, 2048, 24), (1, 3000, 7), (3, 1100, 130)])
+def test_gates_whose_products_leave_float32(torch_mod, shape, reverse):
+    """256 steps that grow by 2^150 and 256 that shrink by as much: states stay within float32, products over either do not"""
+    torch = torch_mod
+    B, T, C = shape
+    g = gen(torch, 2)
+    r = lambda *s: torch.rand(*s, generator=g, device="cuda") + 0.5  # noqa: E731
+    place = torch.arange(T, device="cuda")
+    gate = torch.where(place // 256 % 2 == 0, 1.5, 1 / 1.5)[None, :, None].expand(shape).contiguous()
+    x, dh = 1e-16 * r(*shape), 1e-26 * r(*shape)
+    # what comes back from behind has the steps behind the last whole pair of 256 to go first
+    left = T % 512
+    c = 1e20 * 1.5 ** (-left if left <= 256 else left - 512)      # (its smallest, 1e-25, where the shrinking begins)
+    if reverse:
+        gate, x, dh = (t.flip(1).contiguous() for t in (gate, x, dh))
+    check_walk(torch, x, gate, 1e-15 * r(B, C), dh, c * r(B, C), reverse)
