@@ -60,7 +60,7 @@ def _library():
 def native():
     """The plain calls without Python in between (csrc/seq/sb_seq_torch.cpp): same kernels, same results, a fraction of the host time.
     They answer with an empty list (0) what they do not take; None where the library has not been built, with SB_SEQ_HOST=python, or
-    inside ops.on_stream."""
+    inside ops.on_stream, which the wrappers refuse."""
     lib = _library()
     return lib if lib and not _PYTHON and _OPS._STREAM_OVERRIDE is None else None
 
@@ -93,16 +93,20 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _not_on_stream(name):
+    """Inside ops.on_stream a call's scratch and copies would be made on the current stream and given back to its allocator while the other
+    stream still uses them: refused."""
+    if _OPS._STREAM_OVERRIDE is not None:
+        _fail(f"{name}: not inside ops.on_stream (use torch.cuda.stream)")
+
+
 def _launch(fn, device, *args):
-    """fn(*args, stream) on the tensors' own device and its current stream (ops.on_stream's, inside one)"""
+    """fn(*args, stream) on the tensors' own device and its current stream"""
     index = device.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _launch(fn, device, *args)
-    stream = _OPS._STREAM_OVERRIDE
-    if stream is None:
-        stream = torch._C._cuda_getCurrentRawStream(index)
-    rc = fn(*args, stream)
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         L.check(rc, fn.__name__)
 
@@ -137,6 +141,7 @@ def _norm_params(x, weight, bias):
 def layer_norm_fwd(x, weight, bias, eps=1e-5, stats=True):
     """-> (y, mean, rstd): y = (x - mean) rstd weight + bias over the last axis, x's type; mean and rstd float32 of the leading
     shape (None without `stats`).  weight / bias (None: 1 / 0) in x's type or float32."""
+    _not_on_stream("layer_norm")
     _need(x, "layer_norm: x", _TYPES)
     n = _norm_params(x, weight, bias)
     y = _like(x)
@@ -158,6 +163,7 @@ def layer_norm_fwd(x, weight, bias, eps=1e-5, stats=True):
 def layer_norm_bwd(dy, x, weight, mean, rstd, want_dw=True, want_db=True, wdtype=None, check=True):
     """-> (dx, dw, db) of layer_norm_fwd; dw / db (None where not wanted) in `wdtype` (the weight's, or given for a bias alone),
     summed over the rows in float32 in an order that the shape alone fixes"""
+    _not_on_stream("layer_norm_bwd")
     if check:      # (False: they are layer_norm_fwd's own, and autograd has seen to dy)
         _need(x, "layer_norm_bwd: x", _TYPES)
         _norm_params(x, weight, None)
@@ -199,6 +205,7 @@ def _steps(t, outer, steps, inner):
 
 
 def _scan_sizes(x, gate, dim, form, h0, lengths):
+    _not_on_stream("gated_scan")
     _need(x, "gated_scan: x", _TYPES)
     _need(gate, "gated_scan: gate", (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32), x.device, x.shape)
     if form not in FORMS:
@@ -282,6 +289,7 @@ def gated_scan_bwd(dh, dlast, x, gate, states, *, dim=1, form="sigmoid", reverse
 
 def gated_scan_step(x, gate, state, *, form="sigmoid"):
     """one step: `state` (float32, dense, x's shape) becomes a state + b in place -> its value in x's type"""
+    _not_on_stream("gated_scan_step")
     _need(x, "gated_scan_step: x", _TYPES)
     _need(gate, "gated_scan_step: gate", (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32), x.device, x.shape)
     _need(state, "gated_scan_step: state", (torch.float32,), x.device, x.shape)
@@ -417,6 +425,7 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
     lr: a number or a float32 tensor of one element.  clip > 0: the gradients, scaled by gscale, are clipped to that norm over all
     tensors.  seed: of the 8-bit states' rounding.  skipped: counts a step that the device's watchdog word turned into a no-op
     (ops.adam_step)."""
+    _not_on_stream("adamw_step")
     params, grads = list(params), list(grads)
     step_dev = lr_dev = None
     if isinstance(step, torch.Tensor):
