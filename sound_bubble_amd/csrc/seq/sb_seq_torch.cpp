@@ -3,8 +3,8 @@
 // backward pass that is Python costs a change of thread and interpreter on top.
 //
 // These are the plain calls only.  Whatever is out of the ordinary -- a wrong type, nothing to compute, a copy that Python has to decide on --
-// is "not taken" (an empty list, 0): sound_bubble_amd/ops_seq.py then handles it, or says what is wrong.  The entry points' addresses come
-// from there too (bind), so that one library serves both.
+// is "not taken" (an empty list, 0) before anything is launched: sound_bubble_amd/ops_seq.py then handles it, or says what is wrong.  What
+// is raised is raised for good: nobody runs the call again.  The entry points' addresses come from there too (bind), so that one library serves both.
 //
 // Layer norm and scan are operators of the dispatcher (0.7 us a call).  AdamW's lists of tensors are not: a step over 160 parameters is 39 us of
 // host time by the dispatcher, 18 by the module's function.
@@ -66,7 +66,7 @@ template <class T = void> T* ptr(const Tensor& t) { return t.defined() ? (T*)t.d
 Tensor f32(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kFloat)); }
 Tensor dense_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with status ", rc); }
+void check(int rc, const char* what) { TORCH_CHECK(rc == 0, "sound_bubble: ", what, " failed with status ", rc); }
 
 // passes `value` on and refuses its gradient: the second derivative that there is none of
 struct NoSecond : torch::autograd::Function<NoSecond> {
@@ -320,7 +320,7 @@ std::vector<Tensor> gated_scan_step(const Tensor& x, const Tensor& gate, const T
   Tensor y = dense_like(x);
   const auto [xr, ldx] = rows_of(x, n);
   const auto [gr, ldg] = rows_of(gate, n);
-  state.unsafeGetTensorImpl()->bump_version();
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
   check(entry.gated_scan_step(ptr(xr), ptr(gr), ptr<float>(state), ptr(y), x.numel() / n, n, ldx, ldg, type_of(x), type_of(gate), (int)form, stream_of(x)),
         "sb_gated_scan_step");
   return {y};

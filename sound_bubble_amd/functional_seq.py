@@ -10,6 +10,10 @@ from . import _lib as L
 from . import ops_seq
 
 
+_T, _M, _N = torch.Tensor, (torch.Tensor, type(None)), (int, float)
+_KINDS = {"layer_norm": (_T, _M, _M, _N), "gated_scan": (_T, _T, _M, _M, int, int, bool), "gated_scan_step": (_T, _T, _T, int)}
+
+
 def _native(name, *args):
     """the call without Python in between, where it is one of the plain ones; empty: not taken, the wrappers see to it or say what is
     wrong"""
@@ -19,9 +23,9 @@ def _native(name, *args):
     try:
         return getattr(native, name)(*args)
     except (RuntimeError, TypeError) as e:
-        if str(e).startswith("sound_bubble:"):
-            raise L.SoundBubbleHipError(str(e)) from None
-        return ()
+        if not all(isinstance(a, k) and (k is bool or not isinstance(a, bool)) for a, k in zip(args, _KINDS[name])):      # (nothing has been done)
+            return ()
+        raise ops_seq.said(e)
 
 
 def _recorded(*tensors):

@@ -65,6 +65,11 @@ def native():
     return lib if lib and not _PYTHON and _OPS._STREAM_OVERRIDE is None else None
 
 
+def said(e):
+    """the error to raise for one of the native calls' own: theirs begin with the library's name, others (out of memory, say) stay"""
+    return L.SoundBubbleHipError(str(e)) if str(e).startswith("sound_bubble:") else e
+
+
 def refuse_held_leaves(*leaves):
     """Under capture: raises where an eager graph made on another stream holds one of the leaves (the captured backward pass would
     wait for that stream, which ends the process)."""
@@ -438,13 +443,17 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
     if fast is not None and params and isinstance(state.get("exp_avg"), torch.Tensor):
         bits = 8 if state["exp_avg"].dtype == torch.float8_e4m3fn else 32
         keys = ["exp_avg", "exp_avg_sq"] + ["exp_avg_scale", "exp_avg_sq_scale"] * (bits == 8) + ["master"] * (params[0].dtype != torch.float32)
-        guard = _OPS._SCHED_STATUS.get(params[0].get_device())
+        done = False
         try:
-            done = fast.adamw_step(params, grads, [state[k] for k in keys], bits, step, step_dev, lr, lr_dev, *betas, eps, weight_decay, gscale, clip,
+            buffers = [state[k] for k in keys]
+            guard = _OPS._SCHED_STATUS.get(params[0].get_device())
+            done = fast.adamw_step(params, grads, buffers, bits, step, step_dev, lr, lr_dev, *betas, eps, weight_decay, gscale, clip,
                                    seed & 0xFFFFFFFF, guard.data_ptr() if guard is not None else 0,
                                    skipped.data_ptr() if guard is not None and skipped is not None else 0)
-        except (RuntimeError, TypeError, KeyError, OverflowError):      # (what it is, is said below)
-            done = False
+        except (TypeError, KeyError, OverflowError):      # an argument of another kind, nothing has been done: what it is, is said below
+            pass
+        except RuntimeError as e:      # a launch that failed, perhaps behind others that did not: the step is not begun again
+            raise said(e)
         if done:
             return
     if len(params) != len(grads):

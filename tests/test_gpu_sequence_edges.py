@@ -77,3 +77,19 @@ def test_gates_whose_products_leave_float32(torch_mod, shape, reverse):
     if reverse:
         gate, x, dh = (t.flip(1).contiguous() for t in (gate, x, dh))
     check_walk(torch, x, gate, 1e-15 * r(B, C), dh, c * r(B, C), reverse)
+
+
+# ---- calls out of the ordinary ----
+def test_a_state_made_under_inference_mode(torch_mod):
+    """streaming under no_grad goes on with a state that inference mode made (it has no version count)"""
+    torch = torch_mod
+    from sound_bubble_amd import functional as F
+    x, gate = torch.randn(2, 3, 40, generator=gen(torch, 3), device="cuda")
+    with torch.inference_mode():
+        state = torch.zeros(3, 40, device="cuda")
+        F.gated_scan_step(x, gate, state)
+    with torch.no_grad():
+        y = F.gated_scan_step(x, gate, state)
+    want, _ = F.gated_scan(torch.stack([x, x], 1), torch.stack([gate, gate], 1))
+    assert torch.equal(y, want[:, 1]) and torch.equal(state, want[:, 1])
+    assert torch.equal(F.gated_scan(x[None], gate[None], reverse=1)[0], F.gated_scan(x[None], gate[None], reverse=True)[0])

@@ -15,3 +15,53 @@ def test_refused_inside_on_stream(torch_mod):
     for call in calls:
         with ops.on_stream(1), pytest.raises(E, match="on_stream"):
             call()
+
+
+class Stub:
+    """native calls that have done their work, or the first launch of it, and then raise"""
+
+    def __init__(self, error):
+        self.error, self.calls = error, []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append(name)
+            raise self.error
+        return call
+
+
+@pytest.mark.parametrize("text", ["sound_bubble: sb_adamw_step failed with status -719", "HIP error: unspecified launch failure"])
+def test_a_failed_native_call_is_not_run_again(torch_mod, monkeypatch, text):
+    """an update that has been launched must not be launched a second time by the wrapper"""
+    torch = torch_mod
+    from sound_bubble_amd import _lib as L, functional as F, ops_seq
+    stub, launched = Stub(RuntimeError(text)), []
+    monkeypatch.setattr(ops_seq, "native", lambda: stub)
+    monkeypatch.setattr(ops_seq, "_launch", lambda fn, *a: launched.append(fn))
+    for name in ("layer_norm_fwd", "gated_scan_fwd", "gated_scan_step"):
+        monkeypatch.setattr(ops_seq, name, lambda *a, **k: launched.append(a))
+    x = torch.zeros(2, 3, 4)
+    calls = [lambda: F.layer_norm(x, x[0, 0], None, 1e-5), lambda: F.gated_scan(x, x, reverse=True), lambda: F.gated_scan(x, x, x[:, 0], lengths=x[:, 0, 0]),
+             lambda: F.gated_scan_step(x, x, x.clone(), form="decay"),
+             lambda: ops_seq.adamw_step([x], [x], {"exp_avg": x, "exp_avg_sq": x}, 1, lr=0.1)]
+    for call in calls:
+        with pytest.raises(RuntimeError) as e:
+            call()
+        assert str(e.value) == text and not launched
+        assert isinstance(e.value, L.SoundBubbleHipError) == text.startswith("sound_bubble:")
+    assert stub.calls == ["layer_norm", "gated_scan", "gated_scan", "gated_scan_step", "adamw_step"]
+
+
+def test_arguments_of_another_kind_are_said_to_be(torch_mod, monkeypatch):
+    """what a native call cannot even take (nothing has been done) is for the wrappers to name"""
+    torch = torch_mod
+    from sound_bubble_amd import functional as F, ops_seq
+    from sound_bubble_amd._lib import SoundBubbleHipError as E
+    stub = Stub(TypeError("no such kind"))
+    monkeypatch.setattr(ops_seq, "native", lambda: stub)
+    x = torch.zeros(2, 3, 4)
+    calls = [lambda: F.layer_norm([1.0]), lambda: F.gated_scan(x, None), lambda: F.gated_scan_step(x, x, 3.0),
+             lambda: ops_seq.adamw_step([x], [x], {"exp_avg": x}, 1, lr=0.1), lambda: ops_seq.adamw_step([x], [x], {"exp_avg": x, "exp_avg_sq": x}, 1, lr="0.1")]
+    for call in calls:
+        with pytest.raises(E):
+            call()
