@@ -3,7 +3,7 @@
 // A launch's tensors come as a table in the kernel's arguments; a workgroup takes chunks of kChunk elements, a wave blocks of 256
 // (4 elements a lane), the unit that shares a scale where the states are in 8 bits.  Every operation is rounded by itself (the file is
 // compiled without contraction), so that the value a code is made from is the formula's own; the update itself, which no code is made
-// from, takes the hardware's square root and reciprocal (1 ulp each; v below 2^-126 counts as 0 in it).
+// from, takes the hardware's square root and reciprocal (1 ulp each).
 #include "sb_seq_common.h"
 
 namespace {
@@ -169,6 +169,14 @@ template <class E> SB_DEVINL void stream_store(E* p, const Vec<E, 4>& o) {
   __builtin_nontemporal_store(v, (x4*)p);
 }
 
+// sqrt(v); the hardware's counts v below 2^-126 as 0, which under an eps of 0 makes an infinite update of one of about lr: those are taken
+// 2^64 times as large
+SB_DEVINL float root(float v) {
+  const bool low = v < 1.17549435e-38f;
+  const float s = __builtin_amdgcn_sqrtf(low ? v * 18446744073709551616.f : v);
+  return low ? s * 2.3283064365386963e-10f : s;
+}
+
 // what a lane holds of a block: 4 elements
 template <class P, class G, int BITS> struct Part {
   static constexpr bool kMaster = !std::is_same_v<P, float>;
@@ -208,7 +216,7 @@ template <class P, class G, int BITS> struct Part {
       const float f = (float)g.v[k] * r.gscale;
       m.v[k] = m.v[k] * r.b1 + f * r.c1;
       v.v[k] = v.v[k] * r.b2 + (f * f) * r.c2;
-      p.v[k] = p.v[k] * r.decay - r.rate * (m.v[k] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v.v[k]) * r.root2 + r.eps));
+      p.v[k] = p.v[k] * r.decay - r.rate * (m.v[k] * __builtin_amdgcn_rcpf(root(v.v[k]) * r.root2 + r.eps));
       if (k >= n) m.v[k] = v.v[k] = 0.f;
     }
   }

@@ -1,4 +1,5 @@
 """Sequence-block operators at the edges of their arguments, on the GPU, against their definitions in 64 bits."""
+import numpy as np
 import pytest
 
 from test_gpu_sequence_ops import U, gen, near
@@ -93,3 +94,34 @@ def test_a_state_made_under_inference_mode(torch_mod):
     want, _ = F.gated_scan(torch.stack([x, x], 1), torch.stack([gate, gate], 1))
     assert torch.equal(y, want[:, 1]) and torch.equal(state, want[:, 1])
     assert torch.equal(F.gated_scan(x[None], gate[None], reverse=1)[0], F.gated_scan(x[None], gate[None], reverse=True)[0])
+
+
+# ---- AdamW ----
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-19])
+@pytest.mark.parametrize("pt,bits", [("float32", 32), ("bfloat16", 32), ("float32", 8)])
+def test_adamw_of_tiny_gradients(torch_mod, pt, bits, eps):
+    """v below 2^-126 beside an eps that does not cover it: the update is the formula's, from the kernel's own m and v"""
+    torch = torch_mod
+    from sound_bubble_amd import ops
+    pt = getattr(torch, pt)
+    g = gen(torch, 4)
+    p = torch.randn(3000, generator=g, device="cuda").to(pt)
+    # v = g^2 / 1000 in the first step: 1e-43 .. 1e-35, subnormal up to 1.2e-38
+    grad = 10 ** (-20 + 4 * torch.rand(3000, generator=g, device="cuda")) * torch.randn(3000, generator=g, device="cuda").sign()
+    state = ops.adamw_state([p], bits)
+    lr, wd = 1e-3, 0.01
+    for step in (1, 2, 3):
+        w0 = (state["master"][:3000] if pt != torch.float32 else p).double().cpu().numpy()
+        old = {k: v[:3000].double().cpu().numpy() for k, v in ops.adamw_state_values(state).items()}
+        ops.adamw_step([p], [grad], state, step, lr=lr, eps=eps, weight_decay=wd)
+        m, v = (x[:3000].double().cpu().numpy() for x in ops.adamw_state_values(state).values())
+        if bits == 8:      # (the update goes by the values before their rounding to 8 bits, float32 operations on the decoded ones)
+            f, gr = np.float32, grad.cpu().numpy()
+            m = (old["exp_avg"].astype(f) * f(0.9) + gr * f(1 - 0.9)).astype(np.float64)
+            v = (old["exp_avg_sq"].astype(f) * f(0.999) + (gr * gr) * f(1 - 0.999)).astype(np.float64)
+        assert (v < 2.0 ** -126).sum() > 1000 and (v > 0).all()
+        update = lr / (1 - 0.9 ** step) * m / (np.sqrt(v) / np.sqrt(1 - 0.999 ** step) + eps)
+        got = (state["master"][:3000] if pt != torch.float32 else p).double().cpu().numpy()
+        # root and reciprocal are off by 2 U each, the products, the sum and the rates (rounded to float32) by U: 12 in all; p's own 4
+        bound = 12 * U * np.abs(update) + 4 * U * np.abs(w0)
+        assert (np.abs(got - (w0 * (1 - lr * wd) - update)) <= bound).all()
