@@ -150,8 +150,9 @@ SB_DEVINL Rates rates_of(const sb_adamw_args& a, double* lds) {
   if (a.clip > 0.f) {
     double s = 0.0;
     for (int i = threadIdx.x; i < a.norm_slots; i += 256) s += a.norm_part[i];
-    const float norm = sqrtf((float)block_sum_f64<4>(s, lds)) * a.gscale;
-    const float coef = a.clip / (norm + 1e-6f);
+    s = block_sum_f64<4>(s, lds);
+    // (a sum beyond float32 has a root well within it: finite gradients of 1e20 are clipped, not dropped)
+    const float coef = s > 3.402823466e38 ? (float)(a.clip / (sqrt(s) * a.gscale + 1e-6)) : a.clip / (sqrtf((float)s) * a.gscale + 1e-6f);
     r.gscale *= coef > 1.f ? 1.f : coef;      // (a NaN norm stays one)
   }
   return r;

@@ -125,3 +125,27 @@ def test_adamw_of_tiny_gradients(torch_mod, pt, bits, eps):
         # root and reciprocal are off by 2 U each, the products, the sum and the rates (rounded to float32) by U: 12 in all; p's own 4
         bound = 12 * U * np.abs(update) + 4 * U * np.abs(w0)
         assert (np.abs(got - (w0 * (1 - lr * wd) - update)) <= bound).all()
+
+
+@pytest.mark.parametrize("size", [1e20, 1e30])
+@pytest.mark.parametrize("count", [1, 150])
+def test_clipping_far_beyond_the_norm(torch_mod, count, size):
+    """gradients whose squares' sum leaves float32: they are scaled to the norm that clip asks for"""
+    torch = torch_mod
+    from sound_bubble_amd import ops
+    g = gen(torch, 5)
+    ps = [torch.zeros(700, device="cuda") for _ in range(count)]
+    gs = [size * torch.randn(700, generator=g, device="cuda") for _ in ps]
+    st = ops.adamw_state(ps)
+    ops.adamw_step(ps, gs, st, 1, lr=0.1, clip=2.0, gscale=0.5)
+    flat = torch.cat([t.double() for t in gs]) * 0.5
+    flat *= 2.0 / (flat.norm() + 1e-6)
+    m = torch.cat([st["exp_avg"][768 * k:768 * k + 700] for k in range(count)]).double()
+    v = torch.cat([st["exp_avg_sq"][768 * k:768 * k + 700] for k in range(count)]).double()
+    # the coefficient and its product with gscale: 2 U; two products: 2 U, twice that squared; 1 - beta rounded: U
+    assert ((m - 0.1 * flat).abs() <= 8 * U * 0.1 * flat.abs()).all()
+    assert ((v - 0.001 * flat ** 2).abs() <= 16 * U * 0.001 * flat ** 2 + 2.0 ** -149).all()
+    assert abs(float(m.norm()) / 0.1 - 2.0) < 1e-5
+    gs[0][3] = float("inf")      # (a coefficient of 0, and of it nothing: as torch.nn.utils.clip_grad_norm_)
+    ops.adamw_step(ps, gs, st, 2, lr=0.1, clip=2.0)
+    assert torch.isnan(ps[0][3]) and torch.isfinite(ps[0][4:]).all()
