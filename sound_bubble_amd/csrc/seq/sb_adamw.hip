@@ -100,6 +100,8 @@ template <int M, int BIAS, int TOP> struct Float8 {
   static SB_DEVINL float scale(int byte) {
     return byte == 255 ? __builtin_nanf("") : __int_as_float(byte ? byte << 23 : 1 << 22);
   }
+  // 2^(127 - byte): exact, as the format says (a power function need not be)
+  static SB_DEVINL float inverse(int byte) { return __int_as_float((254 - byte) << 23); }
   // |x| / scale as y >= 0 to a code: up where the part cut off and (u16 + 1/2) / 2^16 reach 1
   static SB_DEVINL unsigned code(float y, unsigned u16) {
     constexpr int CUT = 23 - M;
@@ -112,15 +114,6 @@ template <int M, int BIAS, int TOP> struct Float8 {
 };
 using E4M3 = Float8<3, 7, 8>;
 using E5M2 = Float8<2, 15, 15>;
-
-// 2^(127 - byte), what a block is multiplied by before its codes: powf's value, as torch.ldexp's is, so that a program that packs states
-// with tensor operations gets this kernel's codes.  For 41 of the exponents powf is one ulp below the power of two.  That moves a border
-// between two codes by 2^-24 of the value; a value that is a code's own still becomes it (the half unit that code() adds is 8 or 16 ulp).
-// A workgroup makes the table once, for the 32 blocks and more that it walks.
-SB_DEVINL void fill_inverse(float* inverse) {
-  inverse[threadIdx.x] = powf(2.f, (float)(127 - (int)threadIdx.x));
-  __syncthreads();
-}
 
 struct Rates { float b1, c1, b2, c2, decay, rate, root2, eps, gscale; unsigned key; };
 
@@ -221,7 +214,7 @@ template <class P, class G, int BITS> struct Part {
       if (k >= n) m.v[k] = v.v[k] = 0.f;
     }
   }
-  template <bool FULL> SB_DEVINL void store(const sb_adamw_args& a, const Rates& r, const float* inverse, P* pp, int64_t i, int64_t s, int n) {
+  template <bool FULL> SB_DEVINL void store(const sb_adamw_args& a, const Rates& r, P* pp, int64_t i, int64_t s, int n) {
     if constexpr (kMaster) {
       Vec<P, 4> o;
 #pragma unroll
@@ -242,7 +235,7 @@ template <class P, class G, int BITS> struct Part {
       }
       const int mscale = E4M3::scale_byte(wave_max_bits(mb)), vscale = E5M2::scale_byte(wave_max_bits(vb));
       unsigned mq = 0, vq = 0;
-      const float mi = inverse[mscale], vi = inverse[vscale];
+      const float mi = E4M3::inverse(mscale), vi = E5M2::inverse(vscale);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const unsigned u = dither(s + k, r.key);
@@ -265,12 +258,10 @@ template <class P, class G, int BITS> struct Part {
 template <class P, class G, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(sb_adamw_args a, int chunks) {
   __shared__ double lds[4];
-  __shared__ float inverse[BITS == 8 ? 256 : 1];
   if (a.guard && __hip_atomic_load(a.guard, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0) {
     if (a.last && a.skipped && blockIdx.x == 0 && threadIdx.x == 0) atomicAdd(a.skipped, 1);
     return;
   }
-  if constexpr (BITS == 8) fill_inverse(inverse);
   const Rates r = rates_of(a, lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
@@ -288,13 +279,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(sb_adamw_args a, int chunks)
 #pragma unroll
         for (int b = 0; b < kTogether; ++b) part[b].step(r, 4);
 #pragma unroll
-        for (int b = 0; b < kTogether; ++b) part[b].template store<true>(a, r, inverse, pp, i + b * kBlock, s + b * kBlock, 4);
+        for (int b = 0; b < kTogether; ++b) part[b].template store<true>(a, r, pp, i + b * kBlock, s + b * kBlock, 4);
       } else {
         for (int b = 0; b < kTogether && i0 + (j + b) * kBlock < t.n; ++b) {      // (the whole wave)
           const int n = (int)min(max(t.n - i - b * kBlock, (int64_t)0), (int64_t)4);
           part[0].template load<false>(a, pp, gp, i + b * kBlock, s + b * kBlock, n);
           part[0].step(r, n);
-          part[0].template store<false>(a, r, inverse, pp, i + b * kBlock, s + b * kBlock, n);
+          part[0].template store<false>(a, r, pp, i + b * kBlock, s + b * kBlock, n);
         }
       }
     }

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_sequence_ops import U, gen, near
+from test_gpu_sequence_ops import U, dither, encode, gen, near
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +149,38 @@ def test_clipping_far_beyond_the_norm(torch_mod, count, size):
     gs[0][3] = float("inf")      # (a coefficient of 0, and of it nothing: as torch.nn.utils.clip_grad_norm_)
     ops.adamw_step(ps, gs, st, 2, lr=0.1, clip=2.0)
     assert torch.isnan(ps[0][3]) and torch.isfinite(ps[0][4:]).all()
+
+
+@pytest.mark.parametrize("which", ["exp_avg", "exp_avg_sq"])
+def test_8_bit_codes_at_their_borders(torch_mod, which):
+    """Values whose part cut off and dither add up to exactly 1, in a block of every scale: rounded up, as the format's exact powers of two
+    have it; a scale that is off by one ulp rounds them down.  betas of 0: the moments are g and g^2"""
+    torch = torch_mod
+    from sound_bubble_amd import ops
+    mant, bias, top, lo, hi = (3, 7, 8, 7, 246) if which == "exp_avg" else (2, 15, 15, 15, 239)
+    bytes_, cut, rng = np.arange(lo, hi + 1).repeat(256), 23 - (3 if which == "exp_avg" else 2), np.random.default_rng(1)
+    n = bytes_.size
+    u = dither(n, 1, 0).astype(np.int64)
+    u16 = u & 0xFFFF if which == "exp_avg" else u >> 16
+    add = (u16 << (cut - 16)) + (1 << (cut - 17))
+    g, found = np.zeros(n, np.float32), np.zeros(n, bool)
+    for _ in range(200):      # (not every float32 is a square: other leading bits are tried until one is)
+        e, lead = rng.integers(1 - bias, top, n), rng.integers(0, 1 << mant, n)
+        x = np.ldexp(1 + (lead * 2.0 ** cut + (1 << cut) - add) / 2.0 ** 23, e + bytes_ - 127).astype(np.float32)
+        with np.errstate(over="ignore"):
+            c = x if which == "exp_avg" else np.sqrt(x)
+            ok = ~found & (c.astype(np.float32) == c) & ((c if which == "exp_avg" else c * c) == x)
+        g[ok], found = c[ok], found | ok
+    largest = np.ldexp(1.0, top + bytes_[::256] - 127)      # (1 .. 1.75 of it give this scale)
+    g[::256] = largest if which == "exp_avg" else np.sqrt(largest * np.where((top + bytes_[::256] - 127) % 2, 1.125, 1.0))
+    assert found.mean() > 0.99
+    p = torch.zeros(n, device="cuda")
+    state = ops.adamw_state([p], bits=8)
+    ops.adamw_step([p], [torch.from_numpy(g).cuda()], state, 1, lr=0.1, betas=(0.0, 0.0))
+    exact = np.ldexp(np.float32(1), 127 - np.arange(256))
+    with np.errstate(over="ignore"):
+        want, scale = encode(g if which == "exp_avg" else g * g, exact, mant, bias, top, u16, which != "exp_avg")
+    assert np.array_equal(scale, bytes_[::256].astype(np.uint8))
+    assert np.array_equal(state[which + "_scale"].view(torch.uint8).cpu().numpy(), scale)
+    got = state[which].view(torch.uint8).cpu().numpy()
+    assert np.array_equal(got, want), np.unique(bytes_[got != want])
