@@ -428,7 +428,7 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
     grads: one a parameter, of its type or float32, None: that parameter and its states are left alone.
     step: the step's number, from 1 on -- an int, or an int32 tensor of one element, which a captured graph reads at every replay.
     lr: a number or a float32 tensor of one element.  clip > 0: the gradients, scaled by gscale, are clipped to that norm over all
-    tensors.  seed: of the 8-bit states' rounding.  skipped: counts a step that the device's watchdog word turned into a no-op
+    tensors.  seed: of the 8-bit states' rounding.  skipped (int32, one element): counts a step that the device's watchdog word turned into a no-op
     (ops.adam_step)."""
     _not_on_stream("adamw_step")
     params, grads = list(params), list(grads)
@@ -439,6 +439,9 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
         _fail("adamw_step: a captured graph would repeat this step's number at every replay: pass step as an int32 tensor")
     if isinstance(lr, torch.Tensor):
         lr_dev, lr = lr, 0.0
+    if skipped is not None and not (isinstance(skipped, torch.Tensor) and skipped.dtype is torch.int32 and skipped.is_cuda and skipped.numel() == 1 and
+                                    (not params or skipped.get_device() == params[0].get_device())):      # (the kernel counts it up)
+        _fail("adamw_step: skipped is an int32 tensor of one element on the parameters' GPU")
     fast = native()
     if fast is not None and params and isinstance(state.get("exp_avg"), torch.Tensor):
         bits = 8 if state["exp_avg"].dtype == torch.float8_e4m3fn else 32

@@ -184,3 +184,18 @@ def test_8_bit_codes_at_their_borders(torch_mod, which):
     assert np.array_equal(state[which + "_scale"].view(torch.uint8).cpu().numpy(), scale)
     got = state[which].view(torch.uint8).cpu().numpy()
     assert np.array_equal(got, want), np.unique(bytes_[got != want])
+
+
+def test_adamw_skipped(torch_mod):
+    torch = torch_mod
+    from sound_bubble_amd import ops
+    from sound_bubble_amd._lib import SoundBubbleHipError as E
+    p = torch.ones(300, device="cuda")
+    state = ops.adamw_state([p])
+    for skipped in (torch.zeros(1, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32),
+                    torch.zeros(1, dtype=torch.int64, device="cuda")):
+        with pytest.raises(E, match="skipped"):
+            ops.adamw_step([p], [p.clone()], state, 1, lr=0.1, skipped=skipped)
+    assert p.eq(1).all()
+    ops.adamw_step([p], [p.clone()], state, 1, lr=0.1, skipped=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert not p.eq(1).any()

@@ -65,3 +65,13 @@ def test_arguments_of_another_kind_are_said_to_be(torch_mod, monkeypatch):
     for call in calls:
         with pytest.raises(E):
             call()
+
+
+def test_adamw_refuses_a_counter_that_the_kernel_cannot_count(torch_mod):
+    torch = torch_mod
+    from sound_bubble_amd import ops
+    from sound_bubble_amd._lib import SoundBubbleHipError as E
+    x = torch.zeros(4)
+    for skipped in (torch.zeros(1, dtype=torch.int32), torch.zeros(1), 3):
+        with pytest.raises(E, match="skipped"):
+            ops.adamw_step([x], [x], {}, 1, lr=0.1, skipped=skipped)
