@@ -352,10 +352,14 @@ int adamw_step(const AdamwCall& call) {
       return 0;
     blocks += (p.numel() + SB_ADAMW_BLOCK - 1) / SB_ADAMW_BLOCK;
   }
-  std::vector<const void*> places(count);
-  for (size_t i = 0; i < count; ++i) places[i] = params[i]->data_ptr();
+  std::vector<std::pair<const char*, const char*>> places(count);      // (no two may share memory: their workgroups would race)
+  for (size_t i = 0; i < count; ++i) {
+    const char* at = (const char*)params[i]->data_ptr();
+    places[i] = {at, at + params[i]->nbytes()};
+  }
   std::sort(places.begin(), places.end());
-  if (std::adjacent_find(places.begin(), places.end()) != places.end()) return 0;
+  for (size_t i = 1; i < count; ++i)
+    if (places[i].first < places[i - 1].second) return 0;
   const auto rate = [](double v) { return v >= 0 && v < 1; };
   if (!rate(beta1) || !rate(beta2) || !(eps >= 0)) return 0;
   const size_t buffers = (bits == 8 ? 4 : 2) + (ptype != at::kFloat);

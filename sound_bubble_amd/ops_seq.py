@@ -422,8 +422,8 @@ def _adamw_check_state(state, blocks, device, need_master):
 
 def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, gscale=1.0, clip=0.0, seed=0,
                skipped=None):
-    """One AdamW step (torch.optim.AdamW without amsgrad) over all tensors: `params` and `state` (adamw_state of the same
-    parameters) are updated in place.
+    """One AdamW step (torch.optim.AdamW without amsgrad) over all tensors: `params` (no two updated ones share memory) and `state`
+    (adamw_state of the same parameters) are updated in place.
 
     grads: one a parameter, of its type or float32, None: that parameter and its states are left alone.
     step: the step's number, from 1 on -- an int, or an int32 tensor of one element, which a captured graph reads at every replay.
@@ -504,7 +504,10 @@ def adamw_step(params, grads, state, step, *, lr, betas=(0.9, 0.999), eps=1e-8, 
     if not all(0 <= b < 1 for b in betas) or not eps >= 0:
         _fail(f"adamw_step: betas are in [0, 1) and eps is not negative, got {betas}, {eps}")
     if len({p.data_ptr() for p, n in zip(params, sizes) if n}) < sum(n > 0 for n in sizes):
-        _fail("adamw_step: a parameter is given twice")
+        _fail("adamw_step: a parameter is given twice, or two of them share memory")
+    places = sorted((p.data_ptr(), p.data_ptr() + p.nbytes) for p in ps)
+    if any(a[1] > b[0] for a, b in zip(places, places[1:])):
+        _fail("adamw_step: two parameters share memory")
     if not clip >= 0:
         _fail(f"adamw_step: clip is a norm (0: none), got {clip}")
     if not batches:

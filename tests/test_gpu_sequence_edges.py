@@ -199,3 +199,20 @@ def test_adamw_skipped(torch_mod):
     assert p.eq(1).all()
     ops.adamw_step([p], [p.clone()], state, 1, lr=0.1, skipped=torch.zeros(1, dtype=torch.int32, device="cuda"))
     assert not p.eq(1).any()
+
+
+@pytest.mark.parametrize("how", ["native", "python"])
+def test_adamw_refuses_parameters_that_share_memory(torch_mod, monkeypatch, how):
+    """two workgroups would update the same elements; neighbours in one buffer are fine"""
+    torch = torch_mod
+    from sound_bubble_amd import ops, ops_seq
+    from sound_bubble_amd._lib import SoundBubbleHipError as E
+    monkeypatch.setattr(ops_seq, "_PYTHON", how == "python")
+    flat = torch.ones(1000, device="cuda")
+    for ps in ([flat[:301], flat[300:]], [flat[5:6], flat], [flat, flat[999:]], [flat[:500], flat[500:], flat[200:300]]):
+        with pytest.raises(E, match="share memory"):
+            ops.adamw_step(ps, [p.clone() for p in ps], ops.adamw_state(ps), 1, lr=0.1)
+    assert flat.eq(1).all()
+    ps = [flat[500:], flat[:0], flat[:300], flat[300:500], flat[100:200]]      # (the last one is not updated)
+    ops.adamw_step(ps, [p.clone() for p in ps[:-1]] + [None], ops.adamw_state(ps), 1, lr=0.1)
+    assert not flat.eq(1).any()
