@@ -309,6 +309,15 @@ std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const Maybe&
   const auto [h, last] = scan_fwd(x, gate, or_none(h0), or_none(lengths), z, form, reverse, nullptr);
   return {h, last};
 }
+// rows of a step's input; a copy where they lie on the state's memory in another order, in which other threads write it
+std::pair<Tensor, int64_t> rows_beside(const Tensor& t, const Tensor& state, int64_t n) {
+  auto got = rows_of(t, n);
+  const auto& [r, ld] = got;
+  const char *at = (const char*)r.data_ptr(), *to = (const char*)state.data_ptr();
+  const int64_t size = ((t.numel() / n - 1) * ld + n) * r.element_size();
+  if (at < to + state.nbytes() && to < at + size && !(at == to && ld == n && r.scalar_type() == at::kFloat)) got = {t.clone(at::MemoryFormat::Contiguous), n};
+  return got;
+}
 std::vector<Tensor> gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state, int64_t form) {
   if (!plain(x) || !plain(gate) || !plain(state) || x.numel() == 0 || x.dim() < 1 || gate.sizes() != x.sizes() || state.sizes() != x.sizes() ||
       gate.device() != x.device() || state.device() != x.device() || (gate.scalar_type() != x.scalar_type() && gate.scalar_type() != at::kFloat) ||
@@ -318,8 +327,8 @@ std::vector<Tensor> gated_scan_step(const Tensor& x, const Tensor& gate, const T
   const c10::OptionalDeviceGuard guard(x.device());
   const int64_t n = x.size(-1);
   Tensor y = dense_like(x);
-  const auto [xr, ldx] = rows_of(x, n);
-  const auto [gr, ldg] = rows_of(gate, n);
+  const auto [xr, ldx] = rows_beside(x, state, n);
+  const auto [gr, ldg] = rows_beside(gate, state, n);
   if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
   check(entry.gated_scan_step(ptr(xr), ptr(gr), ptr<float>(state), ptr(y), x.numel() / n, n, ldx, ldg, type_of(x), type_of(gate), (int)form, stream_of(x)),
         "sb_gated_scan_step");

@@ -292,6 +292,16 @@ def gated_scan_bwd(dh, dlast, x, gate, states, *, dim=1, form="sigmoid", reverse
     return dx, dgate, dh0
 
 
+def _rows_beside(t, state, n):
+    """_rows; a copy where they lie on the state's memory in another order, in which other threads write it"""
+    r, ld = _rows(t, n)
+    at, to = r.data_ptr(), state.data_ptr()
+    size = ((t.numel() // n - 1) * ld + n) * r.element_size()
+    if at < to + state.nbytes and to < at + size and not (at == to and ld == n and r.dtype == torch.float32):
+        return t.clone(memory_format=torch.contiguous_format), n
+    return r, ld
+
+
 def gated_scan_step(x, gate, state, *, form="sigmoid"):
     """one step: `state` (float32, dense, x's shape) becomes a state + b in place -> its value in x's type"""
     _not_on_stream("gated_scan_step")
@@ -306,7 +316,7 @@ def gated_scan_step(x, gate, state, *, form="sigmoid"):
     if x.numel() == 0:
         return y
     n = x.shape[-1] if x.dim() else 1
-    (xr, ldx), (gr, ldg) = _rows(x, n), _rows(gate, n)
+    (xr, ldx), (gr, ldg) = _rows_beside(x, state, n), _rows_beside(gate, state, n)
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)
     _launch(L.load().sb_gated_scan_step, x.device, xr.data_ptr(), gr.data_ptr(), state.data_ptr(), y.data_ptr(), x.numel() // n, n, ldx, ldg,

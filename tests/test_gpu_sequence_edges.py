@@ -96,6 +96,28 @@ def test_a_state_made_under_inference_mode(torch_mod):
     assert torch.equal(F.gated_scan(x[None], gate[None], reverse=1)[0], F.gated_scan(x[None], gate[None], reverse=True)[0])
 
 
+@pytest.mark.parametrize("how", ["native", "python"])
+def test_a_step_whose_inputs_are_views_of_its_state(torch_mod, monkeypatch, how):
+    """the inputs are those from before the call, in whatever order they lie on the state's memory"""
+    torch = torch_mod
+    from sound_bubble_amd import functional as F, ops_seq
+    monkeypatch.setattr(ops_seq, "_PYTHON", how == "python")
+    n = 4096
+    views = {"itself": lambda b: b[n:2 * n].view(64, 64), "transposed": lambda b: b[n:2 * n].view(64, 64).t(), "one row": lambda b: b[n:n + 64].expand(64, 64),
+             "behind": lambda b: b[n + 1:2 * n + 1].view(64, 64), "in front": lambda b: b[n - 4:2 * n - 4].view(64, 64),
+             "apart": lambda b: b[2 * n:].view(64, 64), "16 bits": lambda b: b.view(torch.bfloat16)[2 * n:3 * n].view(64, 64)}
+    for name, view in views.items():
+        for gate_too in (False, True):
+            buf = torch.randn(3 * n, generator=gen(torch, 6), device="cuda")
+            state, x = buf[n:2 * n].view(64, 64), view(buf)
+            if name == "16 bits":
+                x.copy_(torch.randn(64, 64, generator=gen(torch, 8), device="cuda"))
+            gate = x if gate_too else torch.randn(64, 64, generator=gen(torch, 7), device="cuda")
+            want = state.clone()
+            y = F.gated_scan_step(x.clone(), gate.clone(), want)
+            assert torch.equal(F.gated_scan_step(x, gate, state), y) and torch.equal(state, want), name
+
+
 # ---- AdamW ----
 @pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-19])
 @pytest.mark.parametrize("pt,bits", [("float32", 32), ("bfloat16", 32), ("float32", 8)])
