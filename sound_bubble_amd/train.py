@@ -231,6 +231,10 @@ class FusedAdamW:
         g0 = groups[0]
         if g0.get("amsgrad", False) or g0.get("maximize", False):
             raise NotImplementedError("amsgrad / maximize optimizer states are not supported")
+        plain = lambda v: tuple(v) if isinstance(v, (list, tuple)) else v  # noqa: E731
+        differ = [k for k in ("lr", "betas", "eps", "weight_decay", "amsgrad", "maximize") if any(plain(g.get(k)) != plain(g0.get(k)) for g in groups)]
+        if differ:
+            raise ValueError(f"parameter groups with {', '.join(differ)} of their own: one group for all parameters is supported")
         values = {k: torch.zeros_like(v) for k, v in ops.adamw_state_values(self.state).items()}
         steps = set()
         for slot, p, o in zip(order, self.params, self.starts):

@@ -238,3 +238,26 @@ def test_adamw_refuses_parameters_that_share_memory(torch_mod, monkeypatch, how)
     ps = [flat[500:], flat[:0], flat[:300], flat[300:500], flat[100:200]]      # (the last one is not updated)
     ops.adamw_step(ps, [p.clone() for p in ps[:-1]] + [None], ops.adamw_state(ps), 1, lr=0.1)
     assert not flat.eq(1).any()
+
+
+@pytest.mark.parametrize("key,value", [("lr", 1e-4), ("weight_decay", 0.0), ("betas", (0.8, 0.999)), ("eps", 1e-6), ("maximize", True)])
+def test_fused_adamw_refuses_states_of_several_groups(torch_mod, key, value):
+    """one group's values would go to all parameters; groups that differ in nothing are fine"""
+    torch = torch_mod
+    from sound_bubble_amd.train import FusedAdamW
+    ps = [torch.nn.Parameter(torch.ones(n, device="cuda")) for n in (30, 5)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt = FusedAdamW(ps, lr=1e-2)
+    opt.step()
+    keep = [t.clone() for t in opt.state.values()]
+    for same in (False, True):
+        other = torch.optim.AdamW([{"params": ps[:1]}, {"params": ps[1:], **({} if same else {key: value})}], lr=1e-3)
+        other.step()
+        if same:
+            opt.load_state_dict(other.state_dict())
+            assert opt.param_groups[0]["lr"] == 1e-3 and opt.step_count == 1
+            continue
+        with pytest.raises(ValueError, match=key):
+            opt.load_state_dict(other.state_dict())
+        assert opt.param_groups[0]["lr"] == 1e-2 and all(torch.equal(a, b) for a, b in zip(keep, opt.state.values()))
