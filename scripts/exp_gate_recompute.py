@@ -36,8 +36,7 @@ def build():
     for name, src, obj, p in procs:
         assert p.wait() == 0, (name, src)
     for name in VARIANTS:
-        objs = [os.path.join(exp, s.replace(".hip", f"_{name}.o")) if s in BF else os.path.join(B.LIBDIR, s.replace(".hip", ".o"))
-                for s in B.SOURCES]
+        objs = B.objects({s: os.path.join(exp, s.replace(".hip", f"_{name}.o")) for s in BF})
         subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o",
                                os.path.join(exp, f"lib_{name}.so")] + objs)
         print("built", name)

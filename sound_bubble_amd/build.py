@@ -74,23 +74,30 @@ PER_FILE_FLAGS = {"sb_lstm_bf_fwd.hip": _BF_FLAGS, "sb_lstm_bf_bwd.hip": _BF_FLA
 EXTRA_UNITS = [("sb_lstm_bf_fwd.hip", "sb_lstm_bf_fwd_2p", _BF_FLAGS + ["-DSB_FWD_2P"])]
 
 
+def object_of(src):
+    """the object of a source, or of the stem of one of EXTRA_UNITS"""
+    return os.path.join(LIBDIR, os.path.basename(src).replace(".hip", "") + ".o")
+
+
+def objects(instead=()):
+    """what libsoundbubble_hip.so is linked from.  instead: {source or stem: another object} of an experiment's library, which has to
+    export all that _lib.load() asks for"""
+    return [dict(instead).get(u, object_of(u)) for u in SOURCES + SEQ_SOURCES + [stem for _, stem, _ in EXTRA_UNITS]]
+
+
 def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     os.makedirs(LIBDIR, exist_ok=True)
-    objs, jobs = [], []
+    objs, jobs = objects(), []
     for src in SOURCES + SEQ_SOURCES:
-        s = os.path.join(CSRC, src)
-        o = os.path.join(LIBDIR, os.path.basename(src).replace(".hip", ".o"))
-        objs.append(o)
+        s, o = os.path.join(CSRC, src), object_of(src)
         if force or _stale(o, [s] + (SEQ_HEADERS if src in SEQ_SOURCES else HEADERS)):
             cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-c", s, "-o", o]
             cmd[2:2] = os.environ.get("SB_EXTRA_HIPCC_FLAGS", "").split()     # e.g. -DSB_PHASE_TIMING (dev tool)
             cmd[2:2] = PER_FILE_FLAGS.get(src, [])
             jobs.append(cmd)
     for src, stem, flags in EXTRA_UNITS:
-        s = os.path.join(CSRC, src)
-        o = os.path.join(LIBDIR, stem + ".o")
-        objs.append(o)
+        s, o = os.path.join(CSRC, src), object_of(stem)
         if force or _stale(o, [s] + HEADERS):
             cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-c", s, "-o", o]
             cmd[2:2] = os.environ.get("SB_EXTRA_HIPCC_FLAGS", "").split()

@@ -1,5 +1,12 @@
 """Sequence-block operators without a GPU: what is refused, and what a failed call leaves behind."""
+import os
+import runpy
+import subprocess
+import sys
+
 import pytest
+
+from conftest import ROOT
 
 
 def test_refused_inside_on_stream(torch_mod):
@@ -75,3 +82,40 @@ def test_adamw_refuses_a_counter_that_the_kernel_cannot_count(torch_mod):
     for skipped in (torch.zeros(1, dtype=torch.int32), torch.zeros(1), 3):
         with pytest.raises(E, match="skipped"):
             ops.adamw_step([x], [x], {}, 1, lr=0.1, skipped=skipped)
+
+
+# ---- the build ----
+class Started:
+    def __init__(self, cmd):
+        self.cmd = cmd
+
+    def wait(self):
+        return 0
+
+
+@pytest.fixture
+def commands(monkeypatch, tmp_path):
+    """the compiler lines of a build into an empty folder, none of them run"""
+    from sound_bubble_amd import build as B
+    got = []
+    for name in ("LIBDIR", "LIB", "TORCH_LIB"):
+        monkeypatch.setattr(B, name, str(tmp_path if name == "LIBDIR" else tmp_path / os.path.basename(getattr(B, name))))
+    monkeypatch.setattr(subprocess, "check_call", lambda cmd, **k: got.append(list(cmd)) or 0)
+    monkeypatch.setattr(subprocess, "Popen", lambda cmd, **k: got.append(list(cmd)) or Started(cmd))
+    return got
+
+
+@pytest.mark.parametrize("script,args,own", [("build_variant.py", ["x", "-DSB_X"], "_x.o"), ("exp_gate_recompute.py", ["build"], "_rc1.o")])
+def test_experiment_libraries_have_every_unit(commands, monkeypatch, script, args, own):
+    """_lib.load() asks a variant of the library for the sequence-block operators' entries too"""
+    from sound_bubble_amd import build as B
+    monkeypatch.setattr(B, "build", lambda *a, **k: None)
+    monkeypatch.setattr(sys, "argv", [script] + args)
+    runpy.run_path(os.path.join(ROOT, "scripts", script), run_name="__main__")
+    links = [c for c in commands if "-shared" in c]
+    assert links
+    units = [os.path.basename(u).replace(".hip", "") for u in B.SOURCES + B.SEQ_SOURCES] + [stem for _, stem, _ in B.EXTRA_UNITS]
+    for link in links:
+        objs = [os.path.basename(o) for o in link if o.endswith(".o")]
+        assert len(objs) == len(units) and all(any(o == u + ".o" or o.startswith(u + "_") for o in objs) for u in units)
+    assert any(o.endswith(own) for link in links for o in link)
