@@ -1,6 +1,8 @@
 """Build libsoundbubble_hip.so (gfx950) in-tree with hipcc -- no torch dependency -- and, beside it, libsoundbubble_torch.so: the
-sequence-block operators' calls from PyTorch (csrc/seq/sb_seq_torch.cpp), host code against the headers of the torch that is installed."""
+sequence-block operators' calls from PyTorch (csrc/seq/sb_seq_torch.cpp), host code against the headers of the torch that is installed.
+Without a torch, a host compiler or Python's headers the first is built alone; the operators then go through their Python wrappers."""
 import os
+import shutil
 import subprocess
 import sys
 
@@ -24,17 +26,42 @@ TORCH_SOURCE = os.path.join(CSRC, "seq", "sb_seq_torch.cpp")
 
 
 def torch_lib_cmd():
-    """the compiler line of libsoundbubble_torch.so (torch is looked up, not imported)"""
+    """-> the compiler line of libsoundbubble_torch.so and a stamp, the line with the torch that it is for (which is looked up, not
+    imported); None and the reason where there is nothing to build it with"""
     import importlib.util
     import sysconfig
-    spec = importlib.util.find_spec("torch")
-    if spec is None:
-        raise RuntimeError("libsoundbubble_torch.so needs an installed torch")
-    t = spec.submodule_search_locations[0]
+    spec, cxx, include = importlib.util.find_spec("torch"), os.environ.get("CXX", "g++").split(), sysconfig.get_paths()["include"]
+    t = spec.submodule_search_locations[0] if spec is not None else ""
+    if not os.path.exists(os.path.join(t, "lib", "libc10_hip.so")):
+        return None, "no torch for ROCm is installed"
+    if shutil.which(cxx[0]) is None:
+        return None, f"no {cxx[0]}"
+    if not os.path.exists(os.path.join(include, "Python.h")):
+        return None, "no Python.h"
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
-    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-D_GLIBCXX_USE_CXX11_ABI=1",
-            "-I" + os.path.join(t, "include"), "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(rocm, "include"),
-            "-I" + sysconfig.get_paths()["include"], TORCH_SOURCE, "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-lamdhip64", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    cmd = [*cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-D_GLIBCXX_USE_CXX11_ABI=1",
+           "-I" + os.path.join(t, "include"), "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(rocm, "include"),
+           "-I" + include, TORCH_SOURCE, "-o", TORCH_LIB, "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_hip", "-lamdhip64", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    with open(os.path.join(t, "version.py")) as f:
+        return cmd, " ".join(cmd) + "\n" + f.read()
+
+
+def _torch_job(force):
+    """-> the compiler line of libsoundbubble_torch.so if it has to be built, and its stamp.  One that is stale and cannot be built is taken away: its
+    calls' layout need not be the library's any more"""
+    cmd, stamp = torch_lib_cmd()
+    stale = force or _stale(TORCH_LIB, [TORCH_SOURCE, SEQ_HEADERS[-1]])
+    if cmd is None:
+        print(f"[build] libsoundbubble_torch.so is not built: {stamp}", flush=True)
+        if stale and os.path.exists(TORCH_LIB):
+            os.remove(TORCH_LIB)
+        return None, ""
+    if os.path.exists(TORCH_LIB + ".stamp"):
+        with open(TORCH_LIB + ".stamp") as f:
+            stale |= f.read() != stamp
+    else:
+        stale = True
+    return (cmd if stale else None), stamp
 
 
 def csrc_digest():
@@ -103,22 +130,22 @@ def build(force=False, verbose=True):
             cmd[2:2] = os.environ.get("SB_EXTRA_HIPCC_FLAGS", "").split()
             cmd[2:2] = flags
             jobs.append(cmd)
-    if force or _stale(TORCH_LIB, [TORCH_SOURCE, SEQ_HEADERS[-1]]):
-        jobs.append(torch_lib_cmd())
-    if jobs:                                   # translation units are independent: compile them side by side
-        from concurrent.futures import ThreadPoolExecutor
+    torch_job, stamp = _torch_job(force)
 
-        def run(cmd):
-            if verbose:
-                print("[build]", " ".join(cmd), flush=True)
-            subprocess.check_call(cmd)
-        with ThreadPoolExecutor(max_workers=min(len(jobs), max(1, (os.cpu_count() or 2) // 2))) as ex:
-            list(ex.map(run, jobs))
-    if force or _stale(LIB, objs):
-        cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
+    def run(cmd):
         if verbose:
             print("[build]", " ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+    from concurrent.futures import ThreadPoolExecutor      # translation units are independent: compile them side by side
+    with ThreadPoolExecutor(max_workers=max(1, min(len(jobs) + 1, (os.cpu_count() or 2) // 2))) as ex:
+        beside = ex.submit(run, torch_job) if torch_job else None
+        list(ex.map(run, jobs))
+        if force or _stale(LIB, objs):
+            run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs)
+        if beside:
+            beside.result()
+            with open(TORCH_LIB + ".stamp", "w") as f:
+                f.write(stamp)
     return LIB
 
 

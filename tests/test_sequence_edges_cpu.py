@@ -119,3 +119,44 @@ def test_experiment_libraries_have_every_unit(commands, monkeypatch, script, arg
         objs = [os.path.basename(o) for o in link if o.endswith(".o")]
         assert len(objs) == len(units) and all(any(o == u + ".o" or o.startswith(u + "_") for o in objs) for u in units)
     assert any(o.endswith(own) for link in links for o in link)
+
+
+@pytest.mark.parametrize("missing", ["torch", "g++", "Python.h"])
+def test_the_library_is_built_without_the_torch_side(commands, monkeypatch, tmp_path, missing):
+    """the C ABI library needs none of them; a stale torch side does not stay beside it"""
+    import importlib.util
+    import shutil
+    import sysconfig
+    from sound_bubble_amd import build as B
+    if missing == "torch":
+        find = importlib.util.find_spec
+        monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else find(name, *a))
+    elif missing == "g++":
+        monkeypatch.setattr(shutil, "which", lambda *a, **k: None)
+    else:
+        monkeypatch.setattr(sysconfig, "get_paths", lambda: {"include": str(tmp_path / "nowhere")})
+    open(B.TORCH_LIB, "w").close()
+    assert B.build(force=True, verbose=False) == B.LIB
+    assert len(commands) == len(B.SOURCES + B.SEQ_SOURCES + B.EXTRA_UNITS) + 1 and "-shared" in commands[-1]
+    assert not any(B.TORCH_SOURCE in c for c in commands) and not os.path.exists(B.TORCH_LIB)
+
+
+def test_the_torch_side_is_built_again_for_another_torch(commands, monkeypatch, tmp_path):
+    import importlib.util
+    from sound_bubble_amd import build as B
+    home = tmp_path / "torch"
+    (home / "lib").mkdir(parents=True)
+    (home / "lib" / "libc10_hip.so").touch()
+    (home / "version.py").write_text("__version__ = '1'")
+    spec = importlib.util.spec_from_loader("torch", None, is_package=True)
+    spec.submodule_search_locations = [str(home)]
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: spec)
+
+    def torch_side():
+        del commands[:]
+        B.build(verbose=False)
+        open(B.TORCH_LIB, "w").close()
+        return sum(B.TORCH_SOURCE in c for c in commands)
+    assert [torch_side(), torch_side()] == [1, 0]
+    (home / "version.py").write_text("__version__ = '2'")
+    assert [torch_side(), torch_side()] == [1, 0]
