@@ -187,10 +187,15 @@ class FusedAdamW:
             step, lr = self._step, self._lr_dev
         else:
             step, lr = self._step + 1, self.param_groups[0]["lr"]
-        with torch.no_grad():
-            ops.adamw_step(self.params, [p.grad for p in self.params], self.state, step, lr=lr, betas=self.betas, eps=self.eps,
-                           weight_decay=self.weight_decay, gscale=1.0 / world_size, clip=float(grad_clip) if grad_clip else 0.0,
-                           seed=self.seed, skipped=self.skipped)
+        try:
+            with torch.no_grad():
+                ops.adamw_step(self.params, [p.grad for p in self.params], self.state, step, lr=lr, betas=self.betas, eps=self.eps,
+                               weight_decay=self.weight_decay, gscale=1.0 / world_size, clip=float(grad_clip) if grad_clip else 0.0,
+                               seed=self.seed, skipped=self.skipped)
+        except ops.L.SoundBubbleHipError:
+            if self.capturable:      # (refused: the step does not count)
+                self._step.sub_(1)
+            raise
         if not self.capturable:
             self._step = step
         bump_weight_epoch()

@@ -261,3 +261,19 @@ def test_fused_adamw_refuses_states_of_several_groups(torch_mod, key, value):
         with pytest.raises(ValueError, match=key):
             opt.load_state_dict(other.state_dict())
         assert opt.param_groups[0]["lr"] == 1e-2 and all(torch.equal(a, b) for a, b in zip(keep, opt.state.values()))
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_does_not_count(torch_mod, capturable):
+    torch = torch_mod
+    from sound_bubble_amd._lib import SoundBubbleHipError as E
+    from sound_bubble_amd.train import FusedAdamW
+    p = torch.nn.Parameter(torch.ones(30, device="cuda").bfloat16())
+    opt = FusedAdamW([p], capturable=capturable)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(E, match="clip"):
+        opt.step(grad_clip=-1.0)
+    assert opt.step_count == 1
+    opt.step()
+    assert opt.step_count == 2
