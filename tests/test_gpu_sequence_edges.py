@@ -2,9 +2,24 @@
 import numpy as np
 import pytest
 
+import test_gpu_sequence_ops as plain
 from test_gpu_sequence_ops import U, dither, encode, gen, near
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- layer norm: groups that take one row after the other ----
+# more than two rows for every group of the forward grid (as many lanes as 4096 waves have, a row's lanes and vectors by its width), and of the
+# backward one; the column sums of wide rows (128 parts) with several rows a part, and with parts that have none
+MANY = [(600001, 1), (150001, 2), (70001, 7), (150001, 8), (40003, 33), (20011, 100), (9001, 255), (9001, 500), (9001, 600), (9001, 1000), (9001, 1500), (4501, 2040),
+        (2501, 1025), (2501, 4096), (2503, 5000), (2503, 8192), (1301, 6100), (1301, 12000), (1301, 16384), (601, 10007), (601, 13001), (601, 20005), (130, 16385),
+        (300, 24576), (129, 24577), (601, 30001), (601, 32768), (1301, 33001), (1100, 40001)]
+
+
+@pytest.mark.parametrize("rows,n", MANY)
+@pytest.mark.parametrize("xt,wt", [("float32", "float32"), ("bfloat16", "bfloat16"), ("float16", "float32")])
+def test_layer_norm_of_many_rows(torch_mod, rows, n, xt, wt):
+    plain.test_layer_norm(torch_mod, rows, n, xt, wt)
 
 
 # ---- gated scan: gates beyond 1 ----
