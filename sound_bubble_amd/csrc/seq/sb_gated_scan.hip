@@ -24,7 +24,7 @@ constexpr int S = 16, kMaxWaves = 8;
 // gate twice.  fp16 6 x 3001 x 1000 (752 waves) forward / backward, us: cut 68 / 94, whole 94 / 134.
 // A segment joins the pairs of all in front of it, 0.1 us each, and walks its own chunks, 2.4 us each in both kernels: of c chunks about
 // 5 sqrt(c) segments.  fp32 1 x 262144 x 16 forward / backward, us: 64 segments 217 / 258, 226 87 / 106; 1 x 65536 x 64: 64 49 / 56, 113 40 / 45.
-// (409 segments: the pairs and powers of as many as 512 pairs alone take.)
+// (409 segments: their pairs and powers take what 512 pairs do)
 constexpr int kFewWaves = 1024, kWaves = 4096, kMaxSplits = 409;
 
 struct Lay {
@@ -181,14 +181,32 @@ template <class E> SB_DEVINL void kill_dead(E (&v)[S], unsigned live) {
 // a state of 0 is NaN where the recurrence stays 0.  It is kept as A 2^power, 0.5 <= |A| < 1 (or 0, infinite, NaN, power whatever), which
 // rounds as the product itself does; the power is taken out every S gates, so that only products of S have to stay within float32.
 SB_DEVINL void take_power(float& A, int& power) {
-  constexpr int kMost = 1 << 24;      // (of a sum: nothing comes back from there within a segment)
-  power = min(max(power + __builtin_amdgcn_frexp_expf(A), -kMost), kMost);
+  power += __builtin_amdgcn_frexp_expf(A);      // (at most 2400 for S gates: 2^31 is 14 M steps of a wave, 10^10 elements and more)
   A = __builtin_amdgcn_frexp_mantf(A);
 }
+SB_DEVINL bool is_normal(int power) { return power >= -125 && power <= 128; }
 // A 2^power c + B; one rounding where A 2^power is a normal number
 SB_DEVINL float join_power(float A, int power, float c, float B) {
-  if (power >= -125 && power <= 128) return __builtin_fmaf(__builtin_ldexpf(A, power), c, B);
+  if (is_normal(power)) return __builtin_fmaf(__builtin_ldexpf(A, power), c, B);
   return __builtin_ldexpf(A * c, power) + B;
+}
+// As it is kept for the second kernel: the product itself where that is a normal number, 0, infinite or NaN.  Where not, its mantissa as the bits
+// of a subnormal number, which nothing else is then (a power of two gets an ulp), with the power beside it.  Behind 1000 any state but 0 is
+// infinite; below 2^-278 any finite one is 0, and so is the product: most of the segments of a sequence that decays.
+// (bf16 1 x 131072 x 512 with fp32 gates, second kernel forward / backward: 97 / 171 us, where powers are read for every segment 101 / 181.)
+constexpr unsigned kSign = 0x80000000u, kFraction = 0x007FFFFFu, kHalf = 126u << 23;
+SB_DEVINL bool is_far(float kept) { return __builtin_amdgcn_classf(kept, 0x90); }      // (subnormal, either sign)
+SB_DEVINL float keep_power(float A, int power, int16_t* at) {
+  const unsigned bits = (unsigned)__float_as_int(A);
+  if (is_normal(power) || (bits & ~(kSign | kFraction)) != kHalf) return __builtin_ldexpf(A, power);
+  if (power <= -278) return 0.f;
+  *at = (int16_t)min(power, 1000);
+  return __int_as_float((int)((bits & kSign) | max(bits & kFraction, 1u)));
+}
+SB_DEVINL float join_kept(float kept, int power, float c, float B) {
+  const float near = __builtin_fmaf(kept, c, B);
+  const float A = __int_as_float((int)((unsigned)__float_as_int(kept) | kHalf));
+  return is_far(kept) ? __builtin_ldexpf(A * c, power) + B : near;
 }
 
 // the pairs of a workgroup's waves, two buffers in turn: [turn][wave][lane]
@@ -212,8 +230,7 @@ struct Pairs {
   }
 };
 
-// k.agg: the segments' pairs [split][A | B][plane], then ("decay") the products' powers [split][plane] in 16 bits: behind +-1000 any
-// state but 0 is infinite, any finite one 0
+// k.agg: the segments' pairs [split][A | B][plane], then ("decay") the powers [split][plane] of products that are far, in 16 bits
 SB_DEVINL int16_t* powers_of(const Kargs& k) { return (int16_t*)(k.agg + 2 * k.splits * k.outer * k.inner); }
 int64_t pairs_floats(int64_t splits, int64_t plane) { return 2 * (splits + (splits + 3) / 4) * plane; }
 
@@ -223,20 +240,41 @@ template <int FORM, bool UP> SB_DEVINL float fold_splits(const float* start, con
   if (!p.on) return 0.f;
   float carry = start ? start[p.q] : 0.f;
   const int n = UP ? split : k.splits - 1 - split;
+  const unsigned at = (unsigned)p.q;      // (time is cut where there are fewer than 2^16 channels)
   constexpr int N = 16;
   for (int j0 = 0; j0 < n; j0 += N) {      // (the loads of N pairs at once: one after the other they cost a trip to memory each)
     float A[N], B[N];
-    int power[N];
+    bool far = false;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int j = UP ? j0 + i : k.splits - 1 - j0 - i;
-      power[i] = FORM == SB_SCAN_DECAY && j0 + i < n ? powers_of(k)[j * plane + p.q] : 0;
-      A[i] = j0 + i < n ? k.agg[(2 * j) * plane + p.q] : 1.f;
-      B[i] = j0 + i < n ? k.agg[(2 * j + 1) * plane + p.q] : 0.f;
+      A[i] = j0 + i < n ? (k.agg + (2 * j) * plane)[at] : 1.f;
+      B[i] = j0 + i < n ? (k.agg + (2 * j + 1) * plane)[at] : 0.f;
+    }
+    if constexpr (FORM == SB_SCAN_DECAY) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) far |= is_far(A[i]);
+    }
+    if (__any(far)) {      // (read again, four at a time: 16 with their powers cost the kernel registers, and with them waves)
+#pragma unroll 1
+      for (int j1 = j0; j1 < min(j0 + N, n); j1 += 4) {
+        float a[4], b[4];
+        int power[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = UP ? min(j1 + i, n - 1) : k.splits - 1 - min(j1 + i, n - 1);
+          a[i] = (k.agg + (2 * j) * plane)[at];
+          b[i] = (k.agg + (2 * j + 1) * plane)[at];
+          power[i] = (powers_of(k) + j * plane)[at];      // (of one that is not far: whatever is there)
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) carry = j1 + i < n ? join_kept(a[i], power[i], carry, b[i]) : carry;
+      }
+      continue;
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (j0 + i < n) carry = FORM == SB_SCAN_DECAY ? join_power(A[i], power[i], carry, B[i]) : __builtin_fmaf(A[i], carry, B[i]);
+      if (j0 + i < n) carry = __builtin_fmaf(A[i], carry, B[i]);
   }
   return carry;
 }
@@ -319,9 +357,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_pair_kernel(Kargs k
   }
   if (p.wave == 0 && p.on) {
     const int64_t plane = k.outer * k.inner;
+    if constexpr (FORM == SB_SCAN_DECAY) whole = keep_power(whole, power, powers_of(k) + split * plane + p.q);
     k.agg[(2 * split) * plane + p.q] = whole;
     k.agg[(2 * split + 1) * plane + p.q] = carry;
-    if constexpr (FORM == SB_SCAN_DECAY) powers_of(k)[split * plane + p.q] = (int16_t)min(max(power, -1000), 1000);
   }
 }
 

@@ -38,14 +38,16 @@ def walk(torch, x, gate, h0, dh, dlast, reverse):
         G[t] = dh[:, t] + c
         c = gate[:, t] * G[t]
     hs, before, G = (torch.stack(v, 1) for v in (hs, before, G))
-    out = {"h": hs, "dx": G, "dgate": G * before}
+    out = {"h": hs, "dx": G, "dgate": G * before, "before": before}
     out = {k: v.flip(1) if reverse else v for k, v in out.items()}
     return {**out, "last": h, "dh0": c}
 
 
 def check_walk(torch, x, gate, h0, dh, dlast, reverse):
     """Every term is positive, so every result is off by the roundings of its terms' factors: a term is a product of at most T gates, T - 1
-    roundings however they are grouped, and as many additions at most; 64 for the joins.  dgate has two such factors."""
+    roundings however they are grouped, and as many additions at most; 64 for the joins.  dgate has two such factors.
+    What is below float32's smallest number is lost: h and G are off by 2^-140 by that (2^10 half steps of 2^-150), and dgate, their product,
+    by 2^-140 of each: a G of 1e-60 beside an h of 1e36 is 0, not 1e-24."""
     from sound_bubble_amd import functional as F, ops_seq
     B, T, C = x.shape
     assert ops_seq._scan_plan(B, T, C, ops_seq._TYPES[x.dtype])[1] > 0, "time is cut at this size"
@@ -56,7 +58,8 @@ def check_walk(torch, x, gate, h0, dh, dlast, reverse):
     want = walk(torch, x, gate, h0, dh, dlast, reverse)
     for k, v in got.items():
         assert want[k].abs().max() < 1e37
-        near(torch, v, want[k], (2 * T + 64) * U * (2 if k == "dgate" else 1) * want[k] + 2.0 ** -140, k)
+        lost = 1 + (want["dx"] + want["before"] if k == "dgate" else 0)
+        near(torch, v, want[k], (2 * T + 64) * U * (2 if k == "dgate" else 1) * want[k] + 2.0 ** -140 * lost, k)
 
 
 @pytest.mark.parametrize("reverse", [False, True])
@@ -93,6 +96,20 @@ def test_gates_whose_products_leave_float32(torch_mod, shape, reverse):
     if reverse:
         gate, x, dh = (t.flip(1).contiguous() for t in (gate, x, dh))
     check_walk(torch, x, gate, 1e-15 * r(B, C), dh, c * r(B, C), reverse)
+
+
+@pytest.mark.parametrize("gate", [2.0 ** -0.5, 0.65, 0.4])
+def test_a_large_state_that_decays_over_segments(torch_mod, gate):
+    """segments whose products are between 2^-278 and 2^-126, or below: what they leave of a state of 1e36 is within float32"""
+    torch = torch_mod
+    g = gen(torch, 9)
+    r = lambda *s: torch.rand(*s, generator=g, device="cuda") + 0.5  # noqa: E731
+    shape = (2, 1100, 24)
+    x, dh = torch.zeros(shape, device="cuda"), torch.zeros(shape, device="cuda")
+    x[:, ::100], dh[:, ::100] = 1e-20 * r(2, 11, 24), 1e-20 * r(2, 11, 24)
+    z = torch.full(shape, gate, device="cuda")
+    # (walk's own small values below float32's are within the 2^-140)
+    check_walk(torch, x, z, 1e36 * r(2, 24), dh, 1e16 * r(2, 24), False)
 
 
 # ---- calls out of the ordinary ----
