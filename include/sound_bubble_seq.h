@@ -87,6 +87,7 @@ int sb_gated_scan_step(const void* x, const void* gate, float* state, void* y, i
  * the block's largest magnitude (448 * 2^k, 57344 * 2^k).  A code is rounded up where the part cut off plus a dither reaches 1 -- a hash of the
  * element's place in the buffer, t and seed -- so that states drift by less than a code's spacing without bias; v > 0 never becomes 0.
  * A block with a NaN or an infinity gets the NaN scale (0xFF).
+ * eps may be 0: a v that is not 0 in float32 counts in the update, subnormal ones too.  No two tensors may share memory.
  * t: step (> 0), or *step_dev; lr: *lr_dev where lr_dev is given. */
 #define SB_ADAMW_BLOCK 256
 #define SB_ADAMW_MAX 112          /* tensors of one launch */
