@@ -329,7 +329,7 @@ extern "C" int sb_adamw_step(const sb_adamw_args* a, void* stream) {
   if (chunks < 0) return (int)chunks;
   if ((a->bits != 32 && a->bits != 8) || !a->m || !a->v || (a->bits == 8 && (!a->m_scale || !a->v_scale))) return -1005;
   if ((a->ptype != SB_F32 && !a->master) || (a->gtype != a->ptype && a->gtype != SB_F32)) return -1006;
-  if ((!a->step_dev && a->step <= 0) || a->clip < 0.f || (a->clip > 0.f && (!a->norm_part || a->norm_slots <= 0 || a->norm_slots > SB_ADAMW_NORM_SLOTS)))
+  if ((!a->step_dev && a->step <= 0) || !(a->clip >= 0.f) || (a->clip > 0.f && (!a->norm_part || a->norm_slots <= 0 || a->norm_slots > SB_ADAMW_NORM_SLOTS)))
     return -1007;
   const int grid = (int)std::min<int64_t>(chunks, kGrid);
   return sb_with_type(a->ptype, [&](auto* pt) -> int {

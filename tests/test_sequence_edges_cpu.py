@@ -84,6 +84,14 @@ def test_adamw_refuses_a_counter_that_the_kernel_cannot_count(torch_mod):
             ops.adamw_step([x], [x], {}, 1, lr=0.1, skipped=skipped)
 
 
+def test_the_c_entry_refuses_a_clip_that_is_no_number(torch_mod):
+    """(it counted as none)"""
+    from sound_bubble_amd import _lib as L
+    a = L.AdamwArgs(count=1, bits=32, m=64, v=64, step=1, clip=float("nan"))      # (64: never looked at, the refusal is the host's)
+    a.t[0] = L.AdamwTensor(64, 64, 10, 0, 0)
+    assert L.load().sb_adamw_step(a, None) <= -1000
+
+
 # ---- the build ----
 class Started:
     def __init__(self, cmd):
