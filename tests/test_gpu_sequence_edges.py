@@ -112,6 +112,26 @@ def test_a_large_state_that_decays_over_segments(torch_mod, gate):
     check_walk(torch, x, z, 1e36 * r(2, 24), dh, 1e16 * r(2, 24), False)
 
 
+def test_as_many_segments_as_there_are(torch_mod):
+    """gates of 1 over 1.2 M steps: sums, forwards and backwards.  A term goes through at most 16 additions in a lane, 8 joins for each of a
+    segment's 24 chunks, or 24 x 16 of a wave's part and 8 joins, and 409 segments: below 1100 roundings"""
+    torch = torch_mod
+    from sound_bubble_amd import functional as F, ops_seq
+    T, C = 1250000, 3
+    assert ops_seq._scan_plan(1, T, C, 0)[1] // (2 * C) == 409 + 103
+    x = (torch.rand(1, T, C, generator=gen(torch, 10), device="cuda") + 0.5).requires_grad_(True)
+    gate = torch.ones(1, T, C, device="cuda", requires_grad=True)
+    h, last = F.gated_scan(x, gate, form="decay")
+    want = x.detach().double().cumsum(1)
+    near(torch, h.detach(), want, 1100 * U * want, "h")
+    dh = torch.rand(1, T, C, generator=gen(torch, 11), device="cuda") + 0.5
+    dx, dgate = torch.autograd.grad(h, (x, gate), dh)
+    G = dh.double().flip(1).cumsum(1).flip(1)
+    near(torch, dx, G, 1100 * U * G, "dx")
+    before = torch.cat([torch.zeros_like(want[:, :1]), want[:, :-1]], 1)
+    near(torch, dgate, G * before, 2201 * U * G * before, "dgate")
+
+
 # ---- calls out of the ordinary ----
 def test_a_state_made_under_inference_mode(torch_mod):
     """streaming under no_grad goes on with a state that inference mode made (it has no version count)"""
